@@ -8,6 +8,7 @@
 #include "common/status.h"
 #include "fused/fused_ops.h"
 #include "gemm/gemm.h"
+#include "head/logprobs.h"
 #include "optim/zero.h"
 #include "peer/peer.h"
 
@@ -508,6 +509,169 @@ void zero_step(const std::vector<int64_t>& grad_ptrs, const std::vector<int64_t>
   check_launch("zero_step");
 }
 
+int logit_type(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  if (t.scalar_type() == torch::kBFloat16) return zx::LOGIT_BF16;
+  if (t.scalar_type() == torch::kFloat16) return zx::LOGIT_FP16;
+  TORCH_CHECK(t.scalar_type() == torch::kFloat32, name, " must be bf16, fp16 or fp32");
+  return zx::LOGIT_FP32;
+}
+void check_logits(const Tensor& t) {
+  TORCH_CHECK(t.dim() == 2 && t.size(1) >= 1 && (t.size(1) == 1 || t.stride(1) == 1),
+              "logits must be [rows, V] with contiguous columns");
+  TORCH_CHECK(t.size(0) <= INT32_MAX && t.size(1) <= zx::kHeadMaxVocab, "logits: at most 2^31 - 1 rows and ",
+              zx::kHeadMaxVocab, " columns");
+}
+// A gradient that is written: rows must not share memory, and it may be the logits but not overlap them otherwise.
+void check_dlogits(const Tensor& d, const Tensor& x) {
+  TORCH_CHECK(d.sizes() == x.sizes() && d.scalar_type() == x.scalar_type() && d.device() == x.device(),
+              "d_logits must have the shape, type and device of the logits");
+  TORCH_CHECK(d.size(1) == 1 || d.stride(1) == 1, "d_logits must have contiguous columns");
+  TORCH_CHECK(d.size(0) <= 1 || d.stride(0) >= d.size(1), "the rows of d_logits share memory");
+  if (d.numel() == 0) return;
+  auto ends = [](const Tensor& t) {
+    const char* p = static_cast<const char*>(t.data_ptr());
+    const int64_t step = t.size(0) > 1 ? t.stride(0) : 0;
+    return std::pair<const char*, const char*>(p, p + ((t.size(0) - 1) * step + t.size(1)) * t.element_size());
+  };
+  const auto a = ends(d), b = ends(x);
+  const bool same = a.first == b.first && (d.size(0) == 1 || d.stride(0) == x.stride(0));
+  TORCH_CHECK(same || a.second <= b.first || b.second <= a.first,
+              "d_logits overlaps the logits without being the same tensor");
+}
+const float* float_rows(const c10::optional<Tensor>& t, int64_t n, const Tensor& like, const char* name) {
+  if (!t.has_value()) return nullptr;
+  TORCH_CHECK(t->device() == like.device() && t->scalar_type() == torch::kFloat32 && t->is_contiguous() && t->numel() == n,
+              name, " must be contiguous fp32 with ", n, " elements on the logits' device");
+  return t->data_ptr<float>();
+}
+float* float_rows(const Tensor& t, int64_t n, const Tensor& like, const char* name) {
+  return const_cast<float*>(float_rows(c10::optional<Tensor>(t), n, like, name));
+}
+zx::IdArray id_array(const Tensor& t, int64_t n, const Tensor& like, const char* name) {
+  TORCH_CHECK(t.device() == like.device() && t.is_contiguous() && t.numel() == n &&
+                  (t.scalar_type() == torch::kInt64 || t.scalar_type() == torch::kInt32),
+              name, " must be contiguous int64 or int32 with ", n, " elements on the logits' device");
+  zx::IdArray a;
+  a.p = t.data_ptr();
+  a.wide = t.scalar_type() == torch::kInt64;
+  return a;
+}
+zx::LogprobsArgs logprobs_args(const Tensor& logits, const c10::optional<Tensor>& targets, const Tensor& entropy,
+                               const Tensor& stats, double temperature) {
+  zx::LogprobsArgs a;
+  a.type = logit_type(logits, "logits");
+  check_logits(logits);
+  TORCH_CHECK(temperature > 0, "the temperature must be positive");
+  a.rows = (int)logits.size(0);
+  a.V = (int)logits.size(1);
+  a.ld = logits.stride(0);
+  a.logits = logits.data_ptr();
+  a.temperature = (float)temperature;
+  if (targets.has_value()) a.targets = id_array(*targets, a.rows, logits, "targets");
+  a.entropy = float_rows(entropy, a.rows, logits, "entropy");
+  a.stats = float_rows(stats, 2 * (int64_t)a.rows, logits, "stats");
+  return a;
+}
+
+// Per row of logits: log-probability of targets (int; outside [0, V): the row is left out), entropy, (maximum, sum of
+// exponentials) in stats, and the top_ids.size(1) most likely columns with their log-probabilities.
+void token_logprobs_fwd(const Tensor& logits, const c10::optional<Tensor>& targets, const c10::optional<Tensor>& logprobs,
+                        Tensor& entropy, Tensor& stats, const c10::optional<Tensor>& top_logprobs,
+                        const c10::optional<Tensor>& top_ids, double temperature) {
+  zx::LogprobsArgs a = logprobs_args(logits, targets, entropy, stats, temperature);
+  TORCH_CHECK(targets.has_value() == logprobs.has_value(), "targets and logprobs come together");
+  a.logprobs = const_cast<float*>(float_rows(logprobs, a.rows, logits, "logprobs"));
+  TORCH_CHECK(top_logprobs.has_value() == top_ids.has_value(), "top_logprobs and top_ids come together");
+  if (top_ids.has_value()) {
+    TORCH_CHECK(top_ids->dim() == 2 && top_ids->size(0) == a.rows && top_ids->size(1) >= 1 &&
+                    top_ids->size(1) <= std::min<int64_t>(a.V, zx::kHeadMaxTop) &&
+                    top_ids->scalar_type() == torch::kInt64, "top_ids must be int64 [rows, 1 .. min(V, ", zx::kHeadMaxTop, ")]");
+    a.top_k = (int)top_ids->size(1);
+    a.top_ids = (int64_t*)id_array(*top_ids, (int64_t)a.rows * a.top_k, logits, "top_ids").p;
+    a.top_logprobs = const_cast<float*>(float_rows(top_logprobs, (int64_t)a.rows * a.top_k, logits, "top_logprobs"));
+  }
+  c10::cuda::CUDAGuard guard(logits.device());
+  a.status = status_ptr();
+  a.sm_count = sm_count();
+  a.stream = cur_stream();
+  zx::launch_token_logprobs_fwd(a);
+  check_launch("token_logprobs_fwd");
+}
+
+// d_logits from the gradients of token_logprobs_fwd's outputs (absent: zero); d_logits may be the logits.
+void token_logprobs_bwd(const Tensor& logits, const c10::optional<Tensor>& targets, const Tensor& entropy,
+                        const Tensor& stats, const c10::optional<Tensor>& top_ids, const c10::optional<Tensor>& d_logprobs,
+                        const c10::optional<Tensor>& d_entropy, const c10::optional<Tensor>& d_top, Tensor& d_logits,
+                        double temperature) {
+  zx::LogprobsArgs a = logprobs_args(logits, targets, entropy, stats, temperature);
+  check_dlogits(d_logits, logits);
+  a.d_logprobs = float_rows(d_logprobs, a.rows, logits, "d_logprobs");
+  a.d_entropy = float_rows(d_entropy, a.rows, logits, "d_entropy");
+  TORCH_CHECK(!d_logprobs.has_value() || targets.has_value(), "d_logprobs needs the targets");
+  if (d_top.has_value()) {
+    TORCH_CHECK(top_ids.has_value() && top_ids->dim() == 2 && top_ids->scalar_type() == torch::kInt64 &&
+                    top_ids->size(1) >= 1 && top_ids->size(1) <= zx::kHeadMaxTop, "d_top needs top_ids int64 [rows, K]");
+    a.top_k = (int)top_ids->size(1);
+    a.top_ids = (int64_t*)id_array(*top_ids, (int64_t)a.rows * a.top_k, logits, "top_ids").p;
+    a.d_top = float_rows(d_top, (int64_t)a.rows * a.top_k, logits, "d_top");
+  }
+  a.d_logits = d_logits.data_ptr();
+  a.d_ld = d_logits.stride(0);
+  c10::cuda::CUDAGuard guard(logits.device());
+  a.status = status_ptr();
+  a.sm_count = sm_count();
+  a.stream = cur_stream();
+  zx::launch_token_logprobs_bwd(a);
+  check_launch("token_logprobs_bwd");
+}
+
+// Divergence from a teacher known by values [rows, K] at the columns ids [rows, K] (outside [0, V): absent).
+//   loss and stats: forward;  stats, d_loss and d_logits: backward;  loss and d_logits: both, with grad_scale.
+void distill_topk(const Tensor& logits, const Tensor& values, const Tensor& ids, const c10::optional<Tensor>& loss,
+                  const c10::optional<Tensor>& stats, const c10::optional<Tensor>& d_loss,
+                  const c10::optional<Tensor>& d_logits, double grad_scale, double temperature, bool bucket) {
+  zx::DistillArgs a;
+  a.type = logit_type(logits, "logits");
+  check_logits(logits);
+  TORCH_CHECK(temperature > 0, "the temperature must be positive");
+  a.rows = (int)logits.size(0);
+  a.V = (int)logits.size(1);
+  a.ld = logits.stride(0);
+  a.logits = logits.data_ptr();
+  a.temperature = (float)temperature;
+  TORCH_CHECK(ids.dim() == 2 && ids.size(0) == a.rows && ids.size(1) >= 1 && ids.size(1) <= zx::kHeadMaxTop,
+              "ids must be [rows, 1 .. ", zx::kHeadMaxTop, "]");
+  a.K = (int)ids.size(1);
+  a.ids = id_array(ids, (int64_t)a.rows * a.K, logits, "ids");
+  a.value_type = logit_type(values, "values");
+  TORCH_CHECK(values.device() == logits.device() && values.sizes() == ids.sizes() && values.is_contiguous(),
+              "values must be contiguous with the shape of ids on the logits' device");
+  a.values = values.data_ptr();
+  a.bucket = bucket;
+  a.grad_scale = (float)grad_scale;
+  a.loss = const_cast<float*>(float_rows(loss, a.rows, logits, "loss"));
+  a.stats = const_cast<float*>(float_rows(stats, 4 * (int64_t)a.rows, logits, "stats"));
+  a.d_loss = float_rows(d_loss, a.rows, logits, "d_loss");
+  if (d_logits.has_value()) {
+    check_dlogits(*d_logits, logits);
+    a.d_logits = d_logits->data_ptr();
+    a.d_ld = d_logits->stride(0);
+  }
+  const bool fwd = loss.has_value() && stats.has_value() && !d_loss.has_value() && !d_logits.has_value();
+  const bool bwd = !loss.has_value() && stats.has_value() && d_loss.has_value() && d_logits.has_value();
+  const bool both = loss.has_value() && !stats.has_value() && !d_loss.has_value() && d_logits.has_value();
+  TORCH_CHECK(fwd || bwd || both, "give loss and stats, or stats, d_loss and d_logits, or loss and d_logits");
+  c10::cuda::CUDAGuard guard(logits.device());
+  a.status = status_ptr();
+  a.sm_count = sm_count();
+  a.stream = cur_stream();
+  if (fwd) zx::launch_distill_fwd(a);
+  else if (bwd) zx::launch_distill_bwd(a);
+  else zx::launch_distill_fwd_bwd(a);
+  check_launch("distill_topk");
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -531,6 +695,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("embedding_fwd", &embedding_fwd);
   m.def("embedding_bwd", &embedding_bwd);
   m.def("ce_fwd_bwd", &ce_fwd_bwd);
+  m.def("token_logprobs_fwd", &token_logprobs_fwd);
+  m.def("token_logprobs_bwd", &token_logprobs_bwd);
+  m.def("distill_topk", &distill_topk);
   m.def("kv_quant_e4m3", &kv_quant_e4m3);
   m.def("kv_dequant_e4m3", &kv_dequant_e4m3);
   m.def("adamw", &adamw);

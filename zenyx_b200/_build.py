@@ -31,6 +31,7 @@ CUDA_SOURCES = [
     "attn/attn_fwd.cu",
     "attn/attn_bwd.cu",
     "fused/fused_ops.cu",
+    "head/logprobs.cu",
     "peer/peer_kernels.cu",
     "optim/zero_adamw.cu",
     "noalloc/attn_bwd_static.cu",

@@ -171,14 +171,18 @@ def test_offsets_beyond_32_bits():
     x.copy_(torch.randn(2, V, device="cuda"))
     y = torch.tensor([3, V - 1], device="cuda")
     _check_fwd(x, y, 4)
-    small = x.contiguous()
-    values, ids = token_logprobs(small, top_k=4)[2:]
-    ref, out = torch.empty_like(small), torch.empty_like(small)
-    ref_loss = distill_topk_fwd_bwd_(small, values, ids, 1.0, tail="bucket", temperature=1.5, out=ref)
+    values, ids = token_logprobs(x, top_k=4)[2:]
+    out = torch.empty(2, V, device="cuda", dtype=torch.bfloat16)
+    ref, grad, off, grad_off = oracle.distill(x, values, ids, 1.5, "bucket")
     loss = distill_topk_fwd_bwd_(x, values, ids, 1.0, tail="bucket", temperature=1.5, out=out)
-    assert torch.equal(loss, ref_loss) and torch.equal(out, ref)
+    oracle.check(loss, ref, off, "loss")
+    oracle.check(out, grad, grad_off, "gradient")
+    a = x.detach().requires_grad_(True)
+    (got,) = torch.autograd.grad(distill_topk(a, values, ids, tail="bucket", temperature=1.5).sum(), a)
+    oracle.check(got, grad, grad_off, "gradient of the autograd form")
+    _check_bwd(x, y, 4)
     distill_topk_fwd_bwd_(x, values, ids, 1.0, tail="bucket", temperature=1.5)
-    assert torch.equal(x, ref) and not flat[V:ld].any()
+    assert torch.equal(x, out) and not flat[V:ld].any()
 
 
 def test_many_rows():
@@ -274,14 +278,14 @@ def test_distill_views_leave_their_surroundings_alone():
             x, _, gen = _logits(T, V, dtype, seed=2)
             values, ids = _teacher(x, K, gen)
             ids[3] = -1
-            ref = torch.empty_like(x)
-            loss = distill_topk_fwd_bwd_(x, values, ids, 1.0, tail="bucket", out=ref)
+            # rows at other addresses are summed up in another order: each result is held to the 64-bit form
+            ref, grad, off, grad_off = oracle.distill(x, values, ids, 1.0, "bucket")
             view = big[1:-1, 8 + shift: 8 + shift + V]
-            assert torch.equal(distill_topk_fwd_bwd_(x, values, ids, 1.0, tail="bucket", out=view), loss)
-            oracle.check(view, ref.double(), ref.double().abs() * torch.finfo(dtype).eps, "out elsewhere")
+            oracle.check(distill_topk_fwd_bwd_(x, values, ids, 1.0, tail="bucket", out=view), ref, off, "loss")
+            oracle.check(view, grad, grad_off, "out elsewhere")
             view.copy_(x)
-            distill_topk_fwd_bwd_(view, values, ids, 1.0, tail="bucket")
-            oracle.check(view, ref.double(), ref.double().abs() * torch.finfo(dtype).eps, "in place elsewhere")
+            oracle.check(distill_topk_fwd_bwd_(view, values, ids, 1.0, tail="bucket"), ref, off, "loss")
+            oracle.check(view, grad, grad_off, "in place elsewhere")
             keep = torch.ones_like(big, dtype=torch.bool)
             keep[1:-1, 8 + shift: 8 + shift + V] = False
             assert (big[keep] == 7.0).all()

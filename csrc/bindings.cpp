@@ -562,7 +562,7 @@ zx::LogprobsArgs logprobs_args(const Tensor& logits, const c10::optional<Tensor>
   zx::LogprobsArgs a;
   a.type = logit_type(logits, "logits");
   check_logits(logits);
-  TORCH_CHECK(temperature > 0, "the temperature must be positive");
+  TORCH_CHECK(temperature >= 1e-4 && temperature <= 1e4, "the temperature must lie in [1e-4, 1e4]");
   a.rows = (int)logits.size(0);
   a.V = (int)logits.size(1);
   a.ld = logits.stride(0);
@@ -634,7 +634,7 @@ void distill_topk(const Tensor& logits, const Tensor& values, const Tensor& ids,
   zx::DistillArgs a;
   a.type = logit_type(logits, "logits");
   check_logits(logits);
-  TORCH_CHECK(temperature > 0, "the temperature must be positive");
+  TORCH_CHECK(temperature >= 1e-4 && temperature <= 1e4, "the temperature must lie in [1e-4, 1e4]");
   a.rows = (int)logits.size(0);
   a.V = (int)logits.size(1);
   a.ld = logits.stride(0);

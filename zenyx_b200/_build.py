@@ -32,6 +32,7 @@ CUDA_SOURCES = [
     "attn/attn_bwd.cu",
     "fused/fused_ops.cu",
     "head/logprobs.cu",
+    "head/distill.cu",
     "peer/peer_kernels.cu",
     "optim/zero_adamw.cu",
     "noalloc/attn_bwd_static.cu",

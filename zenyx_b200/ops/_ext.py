@@ -103,6 +103,8 @@ _SITES = {
     31: "peer barrier", 41: "zero_adamw: peer flag",
     4: "gemm: reduce-scatter owner index", 14: "attn_fwd: output row", 15: "attn_fwd: batch index",
     24: "attn_bwd: dK/dV row", 25: "attn_bwd: dQ row",
+    51: "distill: copy of a slice", 52: "distill: slice ready", 53: "distill: slice free", 54: "distill: cluster exchange",
+    55: "distill: next row",
 }
 
 

@@ -20,7 +20,6 @@ Rows and values that stand for nothing:
 """
 from __future__ import annotations
 
-import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -28,7 +27,8 @@ import torch
 from . import _ext
 
 MAX_TOP = 128          # most alternatives of a row
-MAX_VOCAB = 1 << 20    # most columns
+MAX_VOCAB = 400000     # most columns
+MIN_TEMPERATURE, MAX_TEMPERATURE = 1e-4, 1e4
 _NEG = float("-inf")
 
 
@@ -50,8 +50,8 @@ def _check_logits(logits: torch.Tensor, temperature: float) -> None:
         raise TypeError(f"logits are bf16, fp16 or fp32 (fp64 on the CPU), not {logits.dtype}")
     if logits.dim() < 1 or not 1 <= logits.shape[-1] <= MAX_VOCAB:
         raise ValueError(f"logits are [..., V] with 1 <= V <= {MAX_VOCAB}, not {tuple(logits.shape)}")
-    if not (math.isfinite(temperature) and temperature > 0):
-        raise ValueError(f"the temperature is a positive number, not {temperature}")
+    if not MIN_TEMPERATURE <= temperature <= MAX_TEMPERATURE:
+        raise ValueError(f"the temperature lies in [{MIN_TEMPERATURE:g}, {MAX_TEMPERATURE:g}], not {temperature}")
 
 
 def _check_ids(name: str, ids: torch.Tensor, shape, logits: torch.Tensor) -> None:

@@ -417,3 +417,23 @@ def test_refusals():
                 lambda: C.distill_topk(x, v[:2], ids, f, None, None, x, 1.0, 1.0, False)):
         with pytest.raises(RuntimeError):
             bad()
+
+
+@pytest.mark.parametrize("V,rows", [(600, 700), (50257, 90), (128256, 40)])
+def test_distill_runs_of_rows_that_are_left_out(V, rows):
+    """Rows without entries alone, in runs and at the ends, between others: what is known ahead of a row must not wait for it."""
+    x, _, gen = _logits(rows, V, torch.bfloat16, seed=4)
+    values, ids = _teacher(x, 5, gen)
+    ref_grad = torch.empty_like(x)
+    ref = distill_topk_fwd_bwd_(x, values, ids, 1.0, tail="bucket", out=ref_grad)
+    keep = torch.rand(rows, generator=gen, device="cuda") < 0.3
+    keep[:7] = False
+    keep[rows // 2: rows // 2 + 20] = False
+    keep[-9:] = False
+    for mask in (keep, ~keep, torch.zeros_like(keep)):
+        some = ids.masked_fill(~mask[:, None], -1)
+        out = torch.full_like(x, 5.0)
+        loss = distill_topk_fwd_bwd_(x, values, some, 1.0, tail="bucket", out=out)
+        _ext.check_status()
+        assert torch.equal(loss, ref.masked_fill(~mask, 0.0))
+        assert torch.equal(out, ref_grad.masked_fill(~mask[:, None], 0.0))

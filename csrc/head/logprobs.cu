@@ -49,14 +49,34 @@ __device__ __forceinline__ Sums warp_join(Sums a, float c2) {
 // ------------------------------------------------------------------------------------------
 constexpr int kCandidates = 1024;
 
+static_assert(kCandidates >= kMaxCluster * kHeadMaxTop, "the lists of a cluster");
+constexpr int kGroups = 512;    // groups whose vectors are looked at again
+
 struct TopShared {
-  uint64_t list[kCandidates + 4];
+  uint64_t list[kCandidates + 32];
   uint64_t best[kHeadMaxTop];
   uint32_t hist[256];
+  int group[kGroups];     // step and thread
   uint32_t lo;
-  int n, count, above;
+  int n, count, above, groups;
   int warp[kWarps];
 };
+
+// Descending over the lanes of a warp (bitonic).
+template <class Key>
+__device__ __forceinline__ Key warp_sort(Key key) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int size = 2; size <= 32; size *= 2) {
+#pragma unroll
+    for (int o = size / 2; o > 0; o /= 2) {
+      const Key other = __shfl_xor_sync(0xffffffffu, key, o);
+      const bool larger = ((lane & o) == 0) == ((lane & size) == 0 || size == 32);
+      key = larger == (other > key) ? other : key;
+    }
+  }
+  return key;
+}
 
 // A bound with at least k of the block's group maxima at or above it, and few more: a histogram over [lo, hi] (which
 // holds the k-th largest), and again over the bin that holds it while that is crowded. groups: [steps][threads].
@@ -107,45 +127,54 @@ __device__ __forceinline__ uint32_t find_bound(TopShared& sh, const uint32_t* gr
   return lo;
 }
 
-// best[0 .. k) = the k largest of list[0 .. n), in order (0 where there are fewer): each finds its own place.
+// How many of the 32 keys at run (descending) are above key.
+__device__ __forceinline__ int above_in_run(const uint64_t* run, uint64_t key) {
+  int c = 0;
+#pragma unroll
+  for (int step = 16; step > 0; step /= 2)
+    if (run[c + step - 1] > key) c += step;
+  return c + (run[c] > key ? 1 : 0);
+}
+// best[0 .. k) = the k largest of list[0 .. n), in order (0 where there are fewer): runs of 32 are sorted, each by a warp;
+// a member's place is its own in the run plus, in each other run, the number above it. Needs a barrier before.
 __device__ __forceinline__ void rank_list(TopShared& sh, int n, int k) {
-  for (int i = threadIdx.x; i < k; i += blockDim.x) sh.best[i] = 0;
-  if (threadIdx.x < 4) sh.list[n + threadIdx.x] = 0;
+  const int tid = threadIdx.x, nt = blockDim.x, runs = (n + 31) / 32;
+  for (int i = tid; i < k; i += nt) sh.best[i] = 0;
+  for (int i = tid; i < runs * 32; i += nt) sh.list[i] = warp_sort(i < n ? sh.list[i] : (uint64_t)0);
+  if (tid < 32) sh.list[runs * 32 + tid] = 0;      // an empty run behind the last
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+  for (int i = tid; i < runs * 32; i += nt) {
     const uint64_t mine = sh.list[i];
-    int r = 0;
-#pragma unroll 2
-    for (int j = 0; j < n; j += 4) {
-      const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(&sh.list[j]), b = *reinterpret_cast<const ulonglong2*>(&sh.list[j + 2]);
-      r += (a.x > mine) + (a.y > mine) + (b.x > mine) + (b.y > mine);
+    int r = i & 31;
+    if (mine == 0 || r >= k) continue;
+    r = 0;      // (the own run gives the own place)
+    for (int c = 0; c < runs; c += 4) {       // four at once: the searches are chains of loads
+#pragma unroll
+      for (int b = 0; b < 4; ++b) r += above_in_run(&sh.list[min(c + b, runs) * 32], mine);
     }
     if (r < k) sh.best[r] = mine;
   }
   __syncthreads();
 }
 
-// The same of `lists` sorted lists of k each: a member's place is its own plus, in each other list, the number above it.
+// The same of `lists` sorted lists of k each (of the blocks of a cluster).
 __device__ __forceinline__ void merge_lists(TopShared& sh, const uint64_t* list, int lists, int k) {
-  for (int i = threadIdx.x; i < k; i += blockDim.x) sh.best[i] = 0;
+  // The k-th is not below the smallest of the lists' members number ceil(k / lists), nor below any list's last.
+  const int q = (k + lists - 1) / lists;
+  uint64_t least = ~0ull, lo = 1;
+  for (int b = 0; b < lists; ++b) {
+    least = min(least, list[b * k + q - 1]);
+    lo = max(lo, list[b * k + k - 1]);
+  }
+  lo = max(lo, least);
+  if (threadIdx.x == 0) sh.n = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < lists * k; i += blockDim.x) {
-    const uint64_t mine = list[i];
-    if (mine == 0) continue;
-    int r = i % k;
-    for (int c = 0; c < lists && r < k; ++c) {
-      if (c == i / k) continue;
-      int lo = 0, hi = k;
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (list[c * k + mid] > mine) lo = mid + 1;
-        else hi = mid;
-      }
-      r += lo;
-    }
-    if (r < k) sh.best[r] = mine;
+    const uint64_t key = list[i];
+    if (key >= lo) sh.list[atomicAdd(&sh.n, 1)] = key;
   }
   __syncthreads();
+  rank_list(sh, sh.n, k);
 }
 
 // Any input, ties without end: the k-th largest value by its digits (four passes of 8 bits), then everything above it and
@@ -271,8 +300,11 @@ __device__ __forceinline__ void add_group(uint4 (&v)[kUnroll], float M, float c2
   }
 }
 
-// TOP: a thread keeps the maximum of each of its groups (kUnroll vectors) in shared memory. The k-th largest group
-// maximum bounds the k-th largest logit from below, so only groups at or above it (about k of them) are read again.
+// TOP: a thread keeps the maximum of each of its groups (kUnroll vectors) in shared memory. Any bound with k group maxima
+// at or above it bounds the k-th largest logit from below, so only those groups are read again. The first bound comes from
+// the threads' maxima: in each warp the one that ceil(k / warps) of its threads reach, the smallest of these. Where it lets
+// too many groups pass, a histogram of the group maxima gives a better one; where that does not help either (ties,
+// large logits side by side), the k are selected by their digits from all of the row.
 template <class T, bool TOP>
 __global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(LogprobsArgs a, int cluster, int steps) {
   // TOP: TopShared, the keys of the cluster's blocks [cluster][k] (in the first block), the group maxima
@@ -353,12 +385,14 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(LogprobsArgs 
   t = warp_join(t, c2);
   if (lane == 0) sh.part[warp] = t;
   if (TOP) {
-    const uint32_t least = __reduce_min_sync(0xffffffffu, own);
+    const int q = (K + warps - 1) / warps;        // a warp has that many threads?
+    const uint32_t sorted = warp_sort(own);
+    const uint32_t least = __shfl_sync(0xffffffffu, sorted, min(q, 32) - 1);
     if (lane == 0) {
-      sh.least[warp] = least;
+      sh.least[warp] = q <= 32 ? least : 0;
       sh.most[warp] = order_key(t.m);
     }
-    if (tid == 0) top.n = 0;
+    if (tid == 0) top.n = top.groups = 0;
   }
   __syncthreads();
   // What the row as a whole gives, once its sums are in one warp.
@@ -373,21 +407,22 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(LogprobsArgs 
     a.entropy[r] = bad ? nan_f() : (empty ? 0.f : (float)(log_l - kLn2 * (double)b.s / (double)b.l));
     if (y >= 0) a.logprobs[r] = bad ? nan_f() : (empty ? -inf_f() : (float)(kLn2 * rel2_exact(xy, b.m, c2) - log_l));
   };
-  if (warp == warps - 1) {
+  if (cluster > 1) cluster_wait();   // every block of the cluster has started: its shared memory may be written
+  // The last warp's: joins the block's sums.
+  auto join = [&]() {
     Sums b = lane < warps ? sh.part[lane] : Sums{-FLT_MAX, 0.f, 0.f};
     b = warp_join(b, c2);
-    if (cluster == 1) tell(b);
-    else if (lane == 0) sh.part[0] = b;
-  }
-  if (cluster > 1) {
-    cluster_wait();   // every block of the cluster has started: its shared memory may be written
-    if (warp == warps - 1 && lane == 0) {
-      store_to_cta(&sh.cta[rank][0], 0, sh.part[0].m);
-      store_to_cta(&sh.cta[rank][1], 0, sh.part[0].l);
-      store_to_cta(&sh.cta[rank][2], 0, sh.part[0].s);
+    if (cluster == 1) {
+      tell(b);
+    } else if (lane == 0) {
+      store_to_cta(&sh.cta[rank][0], 0, b.m);
+      store_to_cta(&sh.cta[rank][1], 0, b.l);
+      store_to_cta(&sh.cta[rank][2], 0, b.s);
     }
-  }
+  };
+  if (!TOP && warp == warps - 1) join();
   if (TOP) {
+    bool joined = false;
     uint32_t lo = sh.least[0], hi = sh.most[0];
     for (int w = 1; w < warps; ++w) {
       lo = min(lo, sh.least[w]);
@@ -395,18 +430,41 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(LogprobsArgs 
     }
     int n = 0;
     if (!is_bad(key_value(hi)) && hi > kNegInfKey) {   // else this block has no alternatives
-      // the smallest of the threads' maxima has a group of each thread at or above it
-      if (nt < K || lo <= kNegInfKey) lo = kNegInfKey + 1;
-      lo = find_bound(top, groups, steps, lo, hi, K);
+      lo = max(lo, kNegInfKey + 1);
+      auto gather = [&]() {
+        for (int s = 0; s < steps; ++s)
+          if (groups[s * nt + tid] >= lo) {
+            const int at = atomicAdd(&top.groups, 1);
+            if (at < kGroups) top.group[at] = (s << 16) | tid;
+          }
+        __syncthreads();
+      };
+      gather();
+      if (top.groups > min(kGroups, 2 * K + 32)) {
+        lo = find_bound(top, groups, steps, lo, hi, K);     // (barriers between)
+        if (tid == 0) top.groups = 0;
+        __syncthreads();
+        gather();
+      }
       const float bound = key_value(lo);
-      for (int s = 0; s < steps; ++s) {
-        if (groups[s * nt + tid] < lo) continue;
-        const int i = v0 + s * kUnroll * nt + tid;
-        uint4 v[kUnroll];
+      const int total = min(top.groups, kGroups) * kUnroll;
+      // (the last warp has the row's sums to see to meanwhile)
+      const int hands = warps > 1 ? nt - 32 : nt;
+      if (warp == warps - 1) {
+        join();
+        joined = true;
+      }
+      for (int i = tid; i < total && tid < hands; i += 2 * hands) {
+        uint4 v[2];
+        int vec[2];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) v[u] = row.load(i + u * nt, v1);
+        for (int u = 0; u < 2; ++u) {
+          const int at = i + u * hands, g = top.group[min(at, total - 1) / kUnroll];
+          vec[u] = v0 + ((g >> 16) * kUnroll + at % kUnroll) * nt + (g & 0xffff);
+          v[u] = at < total ? row.load(vec[u], v1) : Vec<T>::nothing();
+        }
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
+        for (int u = 0; u < 2; ++u) {
           if (!(Vec<T>::max_of(Vec<T>::max_w(v[u])) >= bound)) continue;
           const T* e = reinterpret_cast<const T*>(&v[u]);
 #pragma unroll
@@ -414,19 +472,20 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(LogprobsArgs 
             const float x = to_f(e[j]);
             if (x >= bound) {
               const int at = atomicAdd(&top.n, 1);
-              if (at < kCandidates) top.list[at] = alt_key(order_key(x), row.col(i + u * nt) + j);
+              if (at < kCandidates) top.list[at] = alt_key(order_key(x), row.col(vec[u]) + j);
             }
           }
         }
       }
       __syncthreads();
       n = top.n;
-      if (n > kCandidates) {
+      if (n > kCandidates || top.groups > kGroups) {
         __syncthreads();
         select_exactly<T>(top, row, v0, v1, K);
         n = top.n;
       }
     }
+    if (warp == warps - 1 && !joined) join();
     rank_list(top, n, K);
     if (cluster > 1)
       for (int k = tid; k < K; k += nt) store_to_cta(&lists[rank * K + k], 0, top.best[k]);

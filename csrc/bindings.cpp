@@ -1,6 +1,7 @@
 // Python bindings of the sm_100a kernels. Tensors are validated here; the kernels themselves see
 // raw pointers, the current CUDA stream and one process-wide Status word.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
@@ -672,6 +673,126 @@ void distill_topk(const Tensor& logits, const Tensor& values, const Tensor& ids,
   check_launch("distill_topk");
 }
 
+// ---- the same as autograd functions (in C++: a step of a small model is mostly host time) ----
+
+// Gradients that have none of their own: an error when somebody asks for it, as torch.autograd's once_differentiable.
+Tensor differentiable_once(const Tensor& g) {
+  if (!at::GradMode::is_enabled()) return g;
+  auto error = std::make_shared<torch::autograd::DelayedError>("this gradient cannot be differentiated again", 1);
+  return (*error)({g.detach().requires_grad_(true)})[0];
+}
+Tensor rows_of(const Tensor& logits) {   // [..., V] -> [rows, V] with contiguous columns
+  Tensor x = logits.dim() == 2 ? logits : logits.reshape({-1, logits.size(-1)});
+  return x.size(1) == 1 || x.stride(1) == 1 ? x : x.contiguous();
+}
+c10::optional<Tensor> fp32_rows(const Tensor& g) {
+  if (!g.defined()) return c10::nullopt;
+  return g.to(torch::kFloat32).contiguous();
+}
+std::vector<int64_t> lead_of(const Tensor& logits) {
+  auto s = logits.sizes().vec();
+  s.pop_back();
+  return s;
+}
+
+struct TokenLogprobsFn : public torch::autograd::Function<TokenLogprobsFn> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits,
+                                                const c10::optional<Tensor>& targets, int64_t top_k, double temperature) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor x = rows_of(logits);
+    auto lead = lead_of(logits);
+    const auto f32 = x.options().dtype(torch::kFloat32);
+    const bool with_y = targets.has_value();
+    const Tensor y = with_y ? targets->contiguous() : Tensor();
+    Tensor entropy = at::empty(lead, f32), stats = at::empty({x.size(0), 2}, f32), lp, top, ids;
+    if (with_y) lp = at::empty(lead, f32);
+    if (top_k > 0) {
+      lead.push_back(top_k);
+      top = at::empty(lead, f32);
+      ids = at::empty(lead, x.options().dtype(torch::kInt64));
+    }
+    auto opt = [](const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; };
+    auto flat = [&](const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t.view({x.size(0), top_k})) : c10::nullopt; };
+    token_logprobs_fwd(x, opt(y), opt(lp), entropy, stats, flat(top), flat(ids), temperature);
+    torch::autograd::variable_list out{entropy};
+    if (with_y) out.push_back(lp);
+    if (top_k > 0) {
+      out.push_back(top);
+      out.push_back(ids);
+      ctx->mark_non_differentiable({ids});
+    }
+    ctx->save_for_backward({logits, y, entropy, ids, stats});
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["top_k"] = top_k;
+    ctx->set_materialize_grads(false);
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &logits = saved[0], &y = saved[1], &entropy = saved[2], &ids = saved[3], &stats = saved[4];
+    const int64_t top_k = ctx->saved_data["top_k"].toInt();
+    const Tensor d_entropy = grads[0], d_lp = y.defined() ? grads[1] : Tensor();
+    const Tensor d_top = top_k > 0 ? grads[y.defined() ? 2 : 1] : Tensor();
+    Tensor d;
+    if (d_entropy.defined() || d_lp.defined() || d_top.defined()) {
+      at::AutoDispatchBelowADInplaceOrView below;
+      const Tensor x = rows_of(logits);
+      d = at::empty(logits.sizes(), x.options());
+      Tensor d2 = d.view({x.size(0), x.size(1)});
+      token_logprobs_bwd(x, y.defined() ? c10::optional<Tensor>(y) : c10::nullopt, entropy, stats,
+                         top_k > 0 ? c10::optional<Tensor>(ids.view({x.size(0), top_k})) : c10::nullopt, fp32_rows(d_lp),
+                         fp32_rows(d_entropy), fp32_rows(d_top), d2, ctx->saved_data["temperature"].toDouble());
+    }
+    return {d.defined() ? differentiable_once(d) : d, Tensor(), Tensor(), Tensor()};
+  }
+};
+using MaybeTensor = c10::optional<Tensor>;
+// (logprobs, entropy, top_logprobs, top_ids) of logits [..., V]
+std::tuple<MaybeTensor, Tensor, MaybeTensor, MaybeTensor> token_logprobs(const Tensor& logits, const MaybeTensor& targets, int64_t top_k,
+                                                                         double temperature) {
+  const auto out = TokenLogprobsFn::apply(logits, targets, top_k, temperature);
+  size_t i = 1;
+  MaybeTensor lp, top, ids;
+  if (targets.has_value()) lp = out[i++];
+  if (top_k > 0) {
+    top = out[i++];
+    ids = out[i++];
+  }
+  return {lp, out[0], top, ids};
+}
+
+struct DistillFn : public torch::autograd::Function<DistillFn> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& logits, const Tensor& values, const Tensor& ids,
+                        double temperature, bool bucket) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor x = rows_of(logits);
+    const auto f32 = x.options().dtype(torch::kFloat32);
+    const int64_t K = ids.size(-1);
+    const Tensor v = values.reshape({x.size(0), K}).contiguous(), k = ids.reshape({x.size(0), K}).contiguous();
+    Tensor loss = at::empty(lead_of(logits), f32), stats = at::empty({x.size(0), 4}, f32);
+    distill_topk(x, v, k, loss, stats, c10::nullopt, c10::nullopt, 1.0, temperature, bucket);
+    ctx->save_for_backward({logits, v, k, stats});
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["bucket"] = bucket;
+    return loss;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    Tensor d;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      const Tensor x = rows_of(saved[0]);
+      d = at::empty(saved[0].sizes(), x.options());
+      distill_topk(x, saved[1], saved[2], c10::nullopt, saved[3], fp32_rows(grads[0]), d.view({x.size(0), x.size(1)}), 1.0,
+                   ctx->saved_data["temperature"].toDouble(), ctx->saved_data["bucket"].toBool());
+    }
+    return {differentiable_once(d), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+Tensor distill_topk_loss(const Tensor& logits, const Tensor& values, const Tensor& ids, double temperature, bool bucket) {
+  return DistillFn::apply(logits, values, ids, temperature, bucket);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -698,6 +819,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("token_logprobs_fwd", &token_logprobs_fwd);
   m.def("token_logprobs_bwd", &token_logprobs_bwd);
   m.def("distill_topk", &distill_topk);
+  m.def("token_logprobs", &token_logprobs);
+  m.def("distill_topk_loss", &distill_topk_loss);
   m.def("kv_quant_e4m3", &kv_quant_e4m3);
   m.def("kv_dequant_e4m3", &kv_dequant_e4m3);
   m.def("adamw", &adamw);

@@ -437,3 +437,41 @@ def test_distill_runs_of_rows_that_are_left_out(V, rows):
         _ext.check_status()
         assert torch.equal(loss, ref.masked_fill(~mask, 0.0))
         assert torch.equal(out, ref_grad.masked_fill(~mask[:, None], 0.0))
+
+
+def test_gradients_of_gradients_are_refused():
+    x, y, gen = _logits(3, 50, torch.float32)
+    values, ids = _teacher(x, 4, gen)
+    for f in (lambda v: token_logprobs(v, y).entropy, lambda v: distill_topk(v, values, ids)):
+        a = x.clone().requires_grad_(True)
+        (g,) = torch.autograd.grad(f(a).sum(), a, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum(), a)
+
+
+def test_logits_changed_before_the_backward_are_noticed():
+    x, y, _ = _logits(3, 50, torch.float32)
+    a = x.clone().requires_grad_(True)
+    b = a * 1.0
+    loss = token_logprobs(b, y).logprobs.sum()
+    b.data.zero_()                     # (not noticed by design of .data)
+    b = a * 1.0
+    loss = token_logprobs(b, y).logprobs.sum()
+    b.mul_(2.0)
+    with pytest.raises(RuntimeError):
+        loss.backward()
+
+
+def test_shapes_of_the_autograd_forms():
+    x, y, gen = _logits(6, 40, torch.bfloat16)
+    values, ids = _teacher(x, 4, gen)
+    a = x.view(2, 3, 40).clone().requires_grad_(True)
+    out = token_logprobs(a, y.view(2, 3), top_k=2)
+    assert out.logprobs.shape == out.entropy.shape == (2, 3) and out.top_ids.shape == (2, 3, 2)
+    loss = distill_topk(a, values.view(2, 3, 4), ids.view(2, 3, 4))
+    assert loss.shape == (2, 3)
+    (g,) = torch.autograd.grad(out.top_logprobs.sum() + loss.sum(), a)
+    assert g.shape == a.shape and g.dtype == a.dtype
+    one = token_logprobs(x[0], y[0], top_k=2)
+    assert one.logprobs.shape == () and one.top_ids.shape == (2,)
+    assert not token_logprobs(x, y).entropy.requires_grad

@@ -44,9 +44,11 @@ class TokenLogprobs(NamedTuple):
 # ------------------------------------------------------------------------------------------------
 
 
+_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
 def _check_logits(logits: torch.Tensor, temperature: float) -> None:
-    types = (torch.bfloat16, torch.float16, torch.float32) + (() if logits.is_cuda else (torch.float64,))
-    if logits.dtype not in types:
+    if logits.dtype not in _TYPES and (logits.is_cuda or logits.dtype != torch.float64):
         raise TypeError(f"logits are bf16, fp16 or fp32 (fp64 on the CPU), not {logits.dtype}")
     if logits.dim() < 1 or not 1 <= logits.shape[-1] <= MAX_VOCAB:
         raise ValueError(f"logits are [..., V] with 1 <= V <= {MAX_VOCAB}, not {tuple(logits.shape)}")
@@ -57,7 +59,7 @@ def _check_logits(logits: torch.Tensor, temperature: float) -> None:
 def _check_ids(name: str, ids: torch.Tensor, shape, logits: torch.Tensor) -> None:
     if ids.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"{name} are int64 or int32, not {ids.dtype}")
-    if tuple(ids.shape) != tuple(shape):
+    if ids.shape != torch.Size(shape):
         raise ValueError(f"{name} have shape {tuple(ids.shape)}, expected {tuple(shape)}")
     if ids.device != logits.device:
         raise ValueError(f"{name} are on {ids.device}, the logits on {logits.device}")
@@ -158,6 +160,8 @@ def token_logprobs_bwd(logits: torch.Tensor, targets: Optional[torch.Tensor], ou
 
 
 class _TokenLogprobsFn(torch.autograd.Function):
+    """CPU tensors; the CUDA form is an autograd function of the extension."""
+
     @staticmethod
     def forward(ctx, logits, targets, top_k, temperature):
         out, stats = token_logprobs_fwd(logits, targets, top_k, temperature)
@@ -195,6 +199,9 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
         raise ValueError(f"ignore_index {ignore_index} is a token")
     if targets is not None:
         _check_ids("targets", targets, shape, logits)
+    if logits.is_cuda:
+        return TokenLogprobs(*_ext.C().token_logprobs(logits, targets, top_k, temperature))
+    if targets is not None:
         targets = targets.reshape(-1)
     lp, entropy, top, ids = _TokenLogprobsFn.apply(_rows(logits), targets, int(top_k), float(temperature))
     return TokenLogprobs(lp.view(shape) if lp is not None else None, entropy.view(shape),
@@ -214,7 +221,7 @@ def _check_teacher(logits, values, ids, tail: str) -> None:
     if not 1 <= K <= MAX_TOP:
         raise ValueError(f"teacher_ids are [..., K] with 1 <= K <= {MAX_TOP}, not {tuple(ids.shape)}")
     _check_ids("teacher_ids", ids, (*logits.shape[:-1], K), logits)
-    if values.dtype not in (torch.bfloat16, torch.float16, torch.float32) + (() if logits.is_cuda else (torch.float64,)):
+    if values.dtype not in _TYPES and (logits.is_cuda or values.dtype != torch.float64):
         raise TypeError(f"teacher_logprobs are bf16, fp16 or fp32, not {values.dtype}")
     if values.shape != ids.shape:
         raise ValueError(f"teacher_logprobs have shape {tuple(values.shape)}, teacher_ids {tuple(ids.shape)}")
@@ -279,32 +286,20 @@ def distill_topk_fwd_bwd_(logits: torch.Tensor, teacher_logprobs: torch.Tensor, 
 
 
 class _DistillFn(torch.autograd.Function):
+    """CPU tensors; the CUDA form is an autograd function of the extension."""
+
     @staticmethod
     def forward(ctx, logits, values, ids, temperature, bucket):
         ctx.meta = (temperature, bucket)
-        if _ext.use_cuda_kernels(logits):
-            values, ids = values.contiguous(), ids.contiguous()
-            loss = torch.empty(logits.shape[0], device=logits.device, dtype=torch.float32)
-            stats = torch.empty(logits.shape[0], 4, device=logits.device, dtype=torch.float32)
-            _ext.C().distill_topk(logits, values, ids, loss, stats, None, None, 1.0, temperature, bucket)
-            ctx.save_for_backward(logits, values, ids, stats)
-            return loss
-        ctx.save_for_backward(logits, values, ids, None)
+        ctx.save_for_backward(logits, values, ids)
         return _distill_torch(_wide(logits), values, ids, temperature, bucket)[0]
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_loss):
-        logits, values, ids, stats = ctx.saved_tensors
-        temperature, bucket = ctx.meta
-        if stats is not None:
-            grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
-            _ext.C().distill_topk(logits, values, ids, None, stats, d_loss.to(torch.float32).contiguous(), grad, 1.0, temperature,
-                                  bucket)
-        else:
-            grad = _distill_torch(_wide(logits), values, ids, temperature, bucket)[1]
-            grad = (grad * d_loss[:, None]).to(logits.dtype)
-        return grad, None, None, None, None
+        logits, values, ids = ctx.saved_tensors
+        grad = _distill_torch(_wide(logits), values, ids, *ctx.meta)[1]
+        return (grad * d_loss[:, None]).to(logits.dtype), None, None, None, None
 
 
 def distill_topk(logits: torch.Tensor, teacher_logprobs: torch.Tensor, teacher_ids: torch.Tensor, *,
@@ -325,6 +320,8 @@ def distill_topk(logits: torch.Tensor, teacher_logprobs: torch.Tensor, teacher_i
     """
     _check_logits(logits, temperature)
     _check_teacher(logits, teacher_logprobs, teacher_ids, tail)
+    if logits.is_cuda:
+        return _ext.C().distill_topk_loss(logits, teacher_logprobs.detach(), teacher_ids, temperature, tail == "bucket")
     K = teacher_ids.shape[-1]
     loss = _DistillFn.apply(_rows(logits), teacher_logprobs.detach().reshape(-1, K), teacher_ids.reshape(-1, K),
                             float(temperature), tail == "bucket")

@@ -268,13 +268,13 @@ struct FwdShared {
 };
 
 // One group of vectors into the running sums (l and s as pairs).
-template <class T, bool Far>
-__device__ __forceinline__ void add_group(uint4 (&v)[kUnroll], float M, float c2, uint64_t (&l2)[2], uint64_t (&s2)[2]) {
+template <class T, bool Far, int U>
+__device__ __forceinline__ void add_group(const uint4 (&v)[U], float M, float c2, uint64_t (&l2)[2], uint64_t (&s2)[2]) {
   const Rel2<Far> rel(M, c2);
   // -inf stays out of the entropy: in bf16 as a large finite number (two at once), which M is far above
   constexpr bool kClampWords = std::is_same<T, __nv_bfloat16>::value && !Far;
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
+  for (int u = 0; u < U; ++u) {
     uint4 w = v[u];
     if (kClampWords) {
       constexpr uint32_t kLow = 0xf149f149u;     // -9.98e29
@@ -346,18 +346,11 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(LogprobsArgs 
   uint32_t* groups = reinterpret_cast<uint32_t*>(lists + (cluster > 1 ? cluster * K : 0));
   Sums t{-FLT_MAX, 0.f, 0.f};
   uint64_t l2[2] = {0, 0}, s2[2] = {0, 0};
-#pragma unroll 1
-  for (int s = 0; s < steps; ++s) {
-    uint4 now[kUnroll];
+  auto add = [&](const auto& v, int s) {
+    constexpr int U = sizeof(v) / sizeof(v[0]);
+    uint32_t mw = Vec<T>::max_w(v[0]);
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) now[u] = buf[u];
-    if (s + 1 < steps) {
-      const int next = v0 + (s + 1) * kUnroll * nt;
-      row.load_group(buf, next, next + tid, nt, v1);
-    }
-    uint32_t mw = Vec<T>::max_w(now[0]);
-#pragma unroll
-    for (int u = 1; u < kUnroll; ++u) mw = Elem<T>::max_w(mw, Vec<T>::max_w(now[u]));
+    for (int u = 1; u < U; ++u) mw = Elem<T>::max_w(mw, Vec<T>::max_w(v[u]));
     const float gm = Vec<T>::max_of(mw);
     if (TOP) groups[s * nt + tid] = order_key(gm);
     const float M = max_nan(t.m, gm);
@@ -371,8 +364,29 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(LogprobsArgs 
       }
       t.m = M;
     }
-    if (is_far(M, c2)) add_group<T, true>(now, M, c2, l2, s2);
-    else add_group<T, false>(now, M, c2, l2, s2);
+    if (is_far(M, c2)) add_group<T, true>(v, M, c2, l2, s2);
+    else add_group<T, false>(v, M, c2, l2, s2);
+  };
+  if (TOP) {
+#pragma unroll 1
+    for (int s = 0; s < steps; ++s) {
+      uint4 now[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) now[u] = buf[u];
+      if (s + 1 < steps) {
+        const int next = v0 + (s + 1) * kUnroll * nt;
+        row.load_group(buf, next, next + tid, nt, v1);
+      }
+      add(now, s);
+    }
+  } else {
+    add(buf, 0);
+#pragma unroll 1
+    for (int i = v0 + kUnroll * nt; i < v1; i += 2 * kUnroll * nt) {
+      uint4 now[2 * kUnroll];
+      row.load_group(now, i, i + tid, nt, v1);
+      add(now, 0);
+    }
   }
   {
     float x0, x1;

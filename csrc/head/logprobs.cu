@@ -532,8 +532,8 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(LogprobsArgs 
 template <class T, bool ENTROPY>
 __global__ void __launch_bounds__(kThreads, 4) logprobs_bwd_kernel(LogprobsArgs a, int segments) {
   constexpr int P = Vec<T>::kPairs;
-  __shared__ int s_id[kHeadMaxTop + 1];
-  __shared__ float s_c[kHeadMaxTop + 1];
+  __shared__ int s_id[kHeadMaxTop + 4];
+  __shared__ float s_c[kHeadMaxTop + 4], s_sum[kWarps];
   const int tid = threadIdx.x, nt = blockDim.x;
   const int r = blockIdx.x / segments;
   const Row<T> row(a.logits, r, a.ld, a.V);
@@ -549,38 +549,36 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_bwd_kernel(LogprobsArgs 
   // entries: the alternatives, then the target
   const int K = a.d_top != nullptr ? a.top_k : 0;
   const bool with_y = a.targets.p != nullptr && a.d_logprobs != nullptr;
-  for (int k = tid; k <= K; k += nt) {
-    int64_t id = -1;
-    float c = 0.f;
-    if (k < K) {
-      id = a.top_ids[(size_t)r * K + k];
-      if (id >= 0 && id < a.V) c = a.d_top[(size_t)r * K + k];
-      else id = -1;
-    } else if (with_y) {
-      id = load_id(a.targets, r);
-      if (id >= 0 && id < a.V) c = a.d_logprobs[r];
-      else id = -1;
-    }
-    s_id[k] = (int)id;
-    s_c[k] = c;
+  const int entries = K + 1;      // a block has more threads
+  int64_t id64 = -1;
+  float c = 0.f;
+  if (tid < K) {
+    id64 = a.top_ids[(size_t)r * K + tid];
+    c = a.d_top[(size_t)r * K + tid];
+  } else if (tid == K && with_y) {
+    id64 = load_id(a.targets, r);
+    c = a.d_logprobs[r];
   }
+  const bool there = id64 >= 0 && id64 < a.V;
+  const int id = there ? (int)id64 : -1;
+  c = there ? c : 0.f;
+  if (tid < kHeadMaxTop + 4) {
+    s_id[tid] = id;
+    s_c[tid] = c;
+  }
+  const float sum = warp_sum(c);
+  if ((tid & 31) == 0) s_sum[tid >> 5] = sum;
   __syncthreads();
   float g = 0.f;
-  for (int k = 0; k <= K; ++k) g += s_c[k];
+  for (int w = 0; w < (entries + 31) / 32; ++w) g += s_sum[w];
   const float it = 1.f / a.temperature, c2 = scale2(a.temperature), inv_l = 1.f / l;
   // -p (g + h (ln p + H)) = 2^d (A + B d)
   const float h = ENTROPY ? a.d_entropy[r] : 0.f;
   const float B = ENTROPY ? -h * (float)kLn2 * inv_l * it : 0.f;
   const float A = -inv_l * it * (ENTROPY ? g + h * (float)((double)a.entropy[r] - log((double)l)) : g);
-  const int id = tid <= K ? s_id[tid] : -1;     // a block has more threads than a row has entries
   const bool mine = id >= 0 && id >= row.col(v0) && id < row.col(v1);
-  float own = 0.f;
-  if (mine) {
-    const float d = fmaxf(rel2(to_f(row.x[id]), m, c2), kLeast);
-    own = ex2(d) * fmaf(B, d, A);
-    for (int k = 0; k <= K; ++k)
-      if (s_id[k] == id) own += s_c[k] * it;
-  }
+  T own = T();
+  if (mine) own = row.x[id];
   __syncthreads();
   const uint64_t B2 = pair(B, B), A2 = pair(A, A);
   const bool block_whole = v0 >= row.first_full && v0 + nt * kGradVecs <= min(v1, row.end_full) && out.vectors;
@@ -609,7 +607,15 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_bwd_kernel(LogprobsArgs 
   if (is_far(m, c2)) dense(Rel2<true>(m, c2));
   else dense(Rel2<false>(m, c2));
   __syncthreads();
-  if (mine) from_f(own, out.p[id]);
+  if (mine) {
+    const float d = fmaxf(rel2(to_f(own), m, c2), kLeast);
+    float v = ex2(d) * fmaf(B, d, A);
+    for (int k = 0; k < entries; k += 4) {     // (-1 behind the last)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v += s_id[k + u] == id ? s_c[k + u] * it : 0.f;
+    }
+    from_f(v, out.p[id]);
+  }
 }
 
 // ------------------------------------------------------------------------------------------
@@ -642,7 +648,7 @@ void launch_fwd(const LogprobsArgs& a) {
 template <class T>
 void launch_bwd(const LogprobsArgs& a) {
   const int vecs = most_vecs<T>(a.logits, a.ld, a.rows, a.V);
-  const int threads = threads_for(vecs, (a.d_top != nullptr ? a.top_k : 0) + 1);
+  const int threads = threads_for(vecs, a.d_top != nullptr ? kHeadMaxTop + 4 : 4);
   const int segments = (vecs + threads * kGradVecs - 1) / (threads * kGradVecs);
   if (a.d_entropy != nullptr) launch(logprobs_bwd_kernel<T, true>, a.rows, segments, false, threads, 0, a.stream, a, segments);
   else launch(logprobs_bwd_kernel<T, false>, a.rows, segments, false, threads, 0, a.stream, a, segments);

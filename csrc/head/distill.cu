@@ -397,28 +397,48 @@ __device__ __forceinline__ void distill_auxiliary(const DistillArgs& a, DistillS
 }
 
 // Vectors of the slice into the running maximum and sum.
+template <class T, int U, class Rel>
+__device__ __forceinline__ void sum_outside(const uint4 (&v)[U], Rel rel, float gap, uint64_t (&l2)[2]) {
+  const float f = ex2(gap);
+  l2[0] = mul2(l2[0], pair(f, f));
+  l2[1] = mul2(l2[1], pair(f, f));
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int q = 0; q < Vec<T>::kPairs; ++q) {
+      float d0, d1;
+      unpair(rel(Vec<T>::get(v[u], q)), d0, d1);
+      l2[q & 1] = add2(l2[q & 1], pair(ex2(d0), ex2(d1)));
+    }
+}
+// The same, for rows that are far from zero (apart, so that it costs the others nothing).
+template <class T>
+__device__ __noinline__ uint64_t far_outside(const uint4* p, int U, float m, float M, uint64_t l, float c2) {
+  uint64_t l2[2] = {l, 0};
+  for (int u = 0; u < U; ++u) {
+    const uint4 v[1] = {p[u * kWorkers]};
+    const float gap = u == 0 ? gap2_far(m, M, c2) : 0.f;
+    if (is_far(M, c2)) sum_outside<T, 1>(v, Rel2<true>(M, c2), gap, l2);
+    else sum_outside<T, 1>(v, Rel2<false>(M, c2), gap, l2);
+  }
+  return add2(l2[0], l2[1]);
+}
 template <class T, int U>
-__device__ __forceinline__ void add_outside(const uint4 (&v)[U], float& m, uint64_t (&l2)[2], float c2) {
+__device__ __forceinline__ void add_outside(const uint4* p, float& m, uint64_t (&l2)[2], float c2) {
+  uint4 v[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) v[u] = p[u * kWorkers];
   uint32_t mw = Vec<T>::max_w(v[0]);
 #pragma unroll
   for (int u = 1; u < U; ++u) mw = Elem<T>::max_w(mw, Vec<T>::max_w(v[u]));
-  const float M = max_nan(m, Vec<T>::max_of(mw));
-  const float f = ex2(gap2(m, M, c2));
-  l2[0] = mul2(l2[0], pair(f, f));
-  l2[1] = mul2(l2[1], pair(f, f));
+  const float M = max_nan(m, Vec<T>::max_of(mw)), R = ref2(M, c2);
+  if (plain_gap(R)) {
+    sum_outside<T, U>(v, Rel2<false>(M, c2), gap2_plain(m, R, c2), l2);
+  } else {
+    l2[0] = far_outside<T>(p, U, m, M, add2(l2[0], l2[1]), c2);
+    l2[1] = 0;
+  }
   m = M;
-  auto sum = [&](auto rel) {
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int q = 0; q < Vec<T>::kPairs; ++q) {
-        float d0, d1;
-        unpair(rel(Vec<T>::get(v[u], q)), d0, d1);
-        l2[q & 1] = add2(l2[q & 1], pair(ex2(d0), ex2(d1)));
-      }
-  };
-  if (is_far(M, c2)) sum(Rel2<true>(M, c2));
-  else sum(Rel2<false>(M, c2));
 }
 
 template <class T, bool WRITE>
@@ -480,15 +500,9 @@ __global__ void __launch_bounds__(kWorkers + 32, 6) distill_kernel(DistillArgs a
         uint64_t l2[2] = {0, 0};
         int i = tid;
 #pragma unroll 1
-        for (; i + 3 * kWorkers < len; i += 4 * kWorkers) {
-          const uint4 v[4] = {stage[i], stage[i + kWorkers], stage[i + 2 * kWorkers], stage[i + 3 * kWorkers]};
-          add_outside<T, 4>(v, mr, l2, c2);
-        }
+        for (; i + 3 * kWorkers < len; i += 4 * kWorkers) add_outside<T, 4>(stage + i, mr, l2, c2);
 #pragma unroll 1
-        for (; i < len; i += kWorkers) {
-          const uint4 v[1] = {stage[i]};
-          add_outside<T, 1>(v, mr, l2, c2);
-        }
+        for (; i < len; i += kWorkers) add_outside<T, 1>(stage + i, mr, l2, c2);
         float x0, x1;
         unpair(add2(l2[0], l2[1]), x0, x1);
         const float M = warp_max_nan(mr);
@@ -525,12 +539,16 @@ __global__ void __launch_bounds__(kWorkers + 32, 6) distill_kernel(DistillArgs a
       const TeacherPart& tp = sh.teacher[xc][(lane & 7) < cluster ? lane & 7 : 0];
       const float tm = (lane & 7) < cluster ? tp.mt : -FLT_MAX;
       mr = warp_max_nan(part.x);
-      const float mt = warp_max_nan<8>(tm);
-      lr = warp_sum(part.y * ex2(gap2(part.x, mr, c2)));
-      const float lt = warp_sum<8>((lane & 7) < cluster ? tp.lt * ex2(gap2(tm, mt, c2)) : 0.f);
-      const float m = max_nan(mr, mt);
-      const float share = ex2(gap2(mr, m, c2));
-      const float l = lt * ex2(gap2(mt, m, c2)) + lr * share;
+      const float m = max_nan(mr, warp_max_nan<8>(tm)), Rr = ref2(mr, c2), R = ref2(m, c2);
+      float lt, share;
+      auto join = [&](float to_mr, float t_to_m, float r_to_m) {
+        lr = warp_sum(part.y * ex2(to_mr));
+        lt = warp_sum<8>((lane & 7) < cluster ? tp.lt * ex2(t_to_m) : 0.f);
+        share = ex2(r_to_m);
+      };
+      if (plain_gap(Rr) && plain_gap(R)) join(gap2_plain(part.x, Rr, c2), gap2_plain(tm, R, c2), gap2_plain(mr, R, c2));
+      else join(gap2_far(part.x, mr, c2), gap2_far(tm, m, c2), gap2_far(mr, m, c2));
+      const float l = lt + lr * share;
       const bool bad = is_bad(m);
       const float inv_l = bad ? nan_f() : (l == 0.f ? 0.f : 1.f / l);
       const float coef = bad ? nan_f() : (lr == 0.f ? 0.f : share * inv_l - q_rest / lr);

@@ -277,7 +277,7 @@ __device__ __forceinline__ void add_group(const uint4 (&v)[U], float M, float c2
   for (int u = 0; u < U; ++u) {
     uint4 w = v[u];
     if (kClampWords) {
-      constexpr uint32_t kLow = 0xf149f149u;     // -9.98e29
+      constexpr uint32_t kLow = 0xf149f149u;     // -9.98e29 (|M| is below 1e11 here)
       w.x = Elem<T>::max_w(w.x, kLow);
       w.y = Elem<T>::max_w(w.y, kLow);
       w.z = Elem<T>::max_w(w.z, kLow);
@@ -353,9 +353,9 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(LogprobsArgs 
     for (int u = 1; u < U; ++u) mw = Elem<T>::max_w(mw, Vec<T>::max_w(v[u]));
     const float gm = Vec<T>::max_of(mw);
     if (TOP) groups[s * nt + tid] = order_key(gm);
-    const float M = max_nan(t.m, gm);
-    {
-      const float d = gap2(t.m, M, c2), f = ex2(d);
+    const float M = max_nan(t.m, gm), R = ref2(M, c2);
+    auto move = [&](float d) {
+      const float f = ex2(d);
       const uint64_t d2 = pair(d, d), f2 = pair(f, f);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -363,9 +363,15 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(LogprobsArgs 
         l2[i] = mul2(l2[i], f2);
       }
       t.m = M;
+    };
+    if (plain_gap(R)) {
+      move(gap2_plain(t.m, R, c2));
+      add_group<T, false>(v, M, c2, l2, s2);
+    } else {
+      move(gap2_far(t.m, M, c2));
+      if (is_far(M, c2)) add_group<T, true>(v, M, c2, l2, s2);
+      else add_group<T, false>(v, M, c2, l2, s2);
     }
-    if (is_far(M, c2)) add_group<T, true>(v, M, c2, l2, s2);
-    else add_group<T, false>(v, M, c2, l2, s2);
   };
   if (TOP) {
 #pragma unroll 1

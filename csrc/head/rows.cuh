@@ -5,8 +5,9 @@
 //
 // Sums of exponentials are held in 32 bits relative to a maximum m of the row's logits: with c2 = log2(e) / temperature,
 // 2^rel(x) with rel(x) = x c2 - ref(m), ref(m) = m c2 rounded. One fused multiply-add a logit; the rounding of ref(m) is
-// in every term alike and cancels, as long as every reader of (m, sum) takes the same ref(m). Where m c2 is so large that
-// the product says nothing (masks of the type's lowest value), rel(x) = (x - m) c2.
+// in every term alike and cancels, as long as every reader of (m, sum) takes the same ref(m). It must be small beside 1,
+// though: rel(m) is that rounding, and 2^rel(m) has to stay near 1. Where |m c2| is 2^20 or more (a row whose mask leaves
+// large negative numbers only), rel(x) = (x - m) c2: two instructions, and ref(m) is the exact product.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -245,7 +246,9 @@ __device__ __forceinline__ int64_t load_id(const IdArray& a, size_t i) {
 // ------------------------------------------------------------------------------------------
 __device__ __forceinline__ float scale2(float temperature) { return (float)(kLog2e / (double)temperature); }
 __device__ __forceinline__ float ref2(float m, float c2) { return __fmul_rn(m, c2); }
-__device__ __forceinline__ bool is_far(float m, float c2) { return !(fabsf(ref2(m, c2)) < 1e30f && fabsf(m) < 1e29f); }
+constexpr float kFar = 1048576.f;
+__device__ __forceinline__ bool is_far(float m, float c2) { return !(fabsf(ref2(m, c2)) < kFar); }
+__device__ __forceinline__ double ref2_exact(float m, float c2) { return is_far(m, c2) ? (double)m * (double)c2 : (double)ref2(m, c2); }
 __device__ __forceinline__ float rel2(float x, float m, float c2) {
   return is_far(m, c2) ? (x - m) * c2 : __fmaf_rn(x, c2, -ref2(m, c2));
 }
@@ -253,11 +256,22 @@ __device__ __forceinline__ double rel2_exact(float x, float m, float c2) {
   return is_far(m, c2) ? ((double)x - (double)m) * (double)c2 : (double)x * (double)c2 - (double)ref2(m, c2);
 }
 // What sums relative to m are worth relative to M >= m: 2^gap.
-__device__ __forceinline__ float gap2(float m, float M, float c2) {
-  return m == M ? 0.f : fmaxf(ref2(m, c2) - ref2(M, c2), kLeast);   // (the maximum of a NaN and kLeast is kLeast)
-}
 __device__ __forceinline__ double gap2_exact(float m, float M, float c2) {
-  return m == M ? 0. : (is_far(m, c2) || is_far(M, c2) ? ((double)m - (double)M) * (double)c2 : (double)ref2(m, c2) - (double)ref2(M, c2));
+  return m == M ? 0. : ref2_exact(m, c2) - ref2_exact(M, c2);
+}
+// Far from zero the rounded products may hide the gap, or be one where there is hardly any. Where M is nearer than
+// plain_gap's limit, an m that is far has a gap beyond kLeast either way.
+__device__ __forceinline__ bool plain_gap(float ref_M) { return fabsf(ref_M) < kFar - 2048.f; }
+__device__ __forceinline__ float gap2_plain(float m, float ref_M, float c2) {
+  return fmaxf(ref2(m, c2) - ref_M, kLeast);   // (the maximum of a NaN and kLeast is kLeast)
+}
+__device__ __forceinline__ float gap2_far(float m, float M, float c2) {
+  auto rounding = [&](float x) { return is_far(x, c2) ? 0.f : __fmaf_rn(x, c2, -ref2(x, c2)); };
+  return m == M ? 0.f : fmaxf(__fmaf_rn(m - M, c2, rounding(M) - rounding(m)), kLeast);
+}
+__device__ __forceinline__ float gap2(float m, float M, float c2) {
+  const float R = ref2(M, c2);
+  return plain_gap(R) ? gap2_plain(m, R, c2) : gap2_far(m, M, c2);
 }
 
 // rel2 of two logits at once; `Far` as is_far(m, c2).

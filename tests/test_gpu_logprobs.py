@@ -475,3 +475,52 @@ def test_shapes_of_the_autograd_forms():
     one = token_logprobs(x[0], y[0], top_k=2)
     assert one.logprobs.shape == () and one.top_ids.shape == (2,)
     assert not token_logprobs(x, y).entropy.requires_grad
+
+
+def _far_rows(V, dtype):
+    """Rows around +-10^k: all alike (what a mask leaves), a few steps of the type apart, and among ordinary logits."""
+    gen = torch.Generator(device="cuda").manual_seed(17)
+    rows = []
+    for a in (1e3, -6e4, 9e5, -2e6, 3e7, -1e9, 2e10, -1e10, 1e13, -1e17, 1e20, -1e25, 1e29, -3e30, -2e38):
+        if abs(a) > torch.finfo(dtype).max:
+            continue
+        steps = torch.randint(0, 4, (V,), generator=gen, device="cuda")
+        rows.append(torch.full((V,), a, device="cuda", dtype=torch.float64))
+        rows.append(a * (1 - steps.double() * torch.finfo(dtype).eps))
+        mixed = torch.randn(V, generator=gen, device="cuda", dtype=torch.float64) * 3
+        rows.append(torch.where(steps == 0, -abs(a), mixed))
+        rows.append(torch.where(torch.arange(V, device="cuda") == V // 2, abs(a), mixed))
+    return torch.stack(rows).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [5, 257, 50257])
+@pytest.mark.parametrize("t", [1.0, 1e-4, 300.0])
+def test_logits_far_from_zero(dtype, V, t):
+    x = _far_rows(V, dtype)
+    y = torch.arange(x.shape[0], device="cuda") % V
+    _check_fwd(x, y, min(V, 9), t)
+    _check_fwd(x, y, 0, t)
+    _check_bwd(x, y, min(V, 9), t)
+    _check_bwd(x, y, 0, t, ("lp",))
+
+
+@pytest.mark.parametrize("tail", ["renormalize", "bucket"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [5, 257, 50257])
+@pytest.mark.parametrize("t", [1.0, 1e-4, 300.0])
+def test_distill_logits_far_from_zero(tail, dtype, V, t):
+    x = _far_rows(V, dtype)
+    T, K = x.shape[0], 4
+    gen = torch.Generator(device="cuda").manual_seed(18)
+    values = torch.log_softmax(torch.randn(T, K + 1, generator=gen, device="cuda"), 1)[:, :K].contiguous()
+    ids = (torch.randint(0, V, (T, 1), generator=gen, device="cuda") + torch.arange(K, device="cuda")) % V
+    ref, grad, off, grad_off = oracle.distill(x, values, ids, t, tail)
+    a = x.clone().requires_grad_(True)
+    loss = distill_topk(a, values, ids, temperature=t, tail=tail)
+    oracle.check(loss, ref, off, "loss")
+    (got,) = torch.autograd.grad(loss.sum(), a)
+    oracle.check(got, grad, grad_off, "gradient")
+    got = torch.empty_like(x)
+    oracle.check(distill_topk_fwd_bwd_(x, values, ids, 1.0, temperature=t, tail=tail, out=got), ref, off, "loss")
+    oracle.check(got, grad, grad_off, "gradient")

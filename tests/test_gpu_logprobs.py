@@ -524,3 +524,13 @@ def test_distill_logits_far_from_zero(tail, dtype, V, t):
     got = torch.empty_like(x)
     oracle.check(distill_topk_fwd_bwd_(x, values, ids, 1.0, temperature=t, tail=tail, out=got), ref, off, "loss")
     oracle.check(got, grad, grad_off, "gradient")
+
+
+def test_logits_overwritten_before_the_backward_are_noticed():
+    x, y, _ = _logits(4, 100, torch.float32)
+    x.requires_grad_(True)
+    z = x * 1.0
+    out = token_logprobs(z, y)
+    distill_topk_fwd_bwd_(z.detach(), torch.zeros(4, 1, device="cuda"), y[:, None], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.logprobs.sum().backward()

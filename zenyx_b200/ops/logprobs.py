@@ -71,6 +71,12 @@ def _rows(logits: torch.Tensor) -> torch.Tensor:
     return x if x.shape[1] == 1 or x.stride(1) == 1 else x.contiguous()
 
 
+def _overwritten(x: torch.Tensor) -> None:
+    """Tells autograd, so that a backward that has kept these logits is an error instead of wrong."""
+    if not x.is_inference():
+        torch.autograd.graph.increment_version(x)
+
+
 def _wide(x: torch.Tensor) -> torch.Tensor:
     return x if x.dtype == torch.float64 else x.float()
 
@@ -137,6 +143,7 @@ def token_logprobs_bwd(logits: torch.Tensor, targets: Optional[torch.Tensor], ou
 
         _ext.C().token_logprobs_bwd(logits, targets.contiguous() if targets is not None else None, out.entropy, stats,
                                     out.top_ids, fp32(d_logprobs), fp32(d_entropy), fp32(d_top), d_logits, temperature)
+        _overwritten(d_logits)
         return d_logits
     x = _wide(logits)
     m, l = stats[:, 0], stats[:, 1]
@@ -279,6 +286,7 @@ def distill_topk_fwd_bwd_(logits: torch.Tensor, teacher_logprobs: torch.Tensor, 
         loss = torch.empty(logits.shape[0], device=logits.device, dtype=torch.float32)
         _ext.C().distill_topk(logits, teacher_logprobs.contiguous(), teacher_ids.contiguous(), loss, None, None, out,
                               grad_scale, temperature, tail == "bucket")
+        _overwritten(out)
         return loss
     loss, grad = _distill_torch(_wide(logits), teacher_logprobs, teacher_ids, temperature, tail == "bucket")
     out.copy_(grad * grad_scale)

@@ -18,13 +18,15 @@ Design points:
   layout, K/V go to peer-visible slots and attention runs through ``ring_attn_forward/backward``.
 
 Two entry points share that code: ``forward_backward`` (the training engine calls it once per
-micro-batch) and ``loss`` (a normal autograd scalar, for ``loss.backward()`` style code).
+micro-batch) and ``loss`` (a normal autograd scalar, for ``loss.backward()`` style code). The chunked head also serves
+``token_logprobs`` (scoring, and writing down a teacher's most likely tokens) and ``forward_backward_distill`` (training
+on what a teacher wrote down).
 """
 from __future__ import annotations
 
 import math
 from dataclasses import dataclass, field
-from typing import Dict, List, Optional, Tuple
+from typing import Callable, Dict, List, Optional, Tuple
 
 import torch
 import torch.nn as nn
@@ -32,6 +34,7 @@ import torch.nn as nn
 from ..ops import fused
 from ..ops.attention import RingContext, ring_attn_backward, ring_attn_forward
 from ..ops.gemm import gemm
+from ..ops.logprobs import TokenLogprobs, distill_topk_fwd_bwd_, token_logprobs
 from ..utils.tracing import trace_range
 
 
@@ -414,7 +417,13 @@ class LlamaModel(nn.Module):
     # -------------------------------------------------------------------------------------------
     # LM head + loss, forward and backward in one sweep over token chunks
     # -------------------------------------------------------------------------------------------
-    def _head_loss(self, h, targets, loss_weight: float, want_grad: bool):
+    def _cross_entropy_head(self, targets, loss_weight: float) -> Callable:
+        tflat = targets.reshape(-1)
+        return lambda logits, t0, t1: fused.cross_entropy_fwd_bwd_(logits, tflat[t0:t1], loss_weight)
+
+    def _head_loss(self, h, chunk_loss: Callable, loss_weight: float, want_grad: bool):
+        """``chunk_loss(logits, t0, t1)`` returns the losses of tokens t0 .. t1 and overwrites their logits with
+        loss_weight times the gradient."""
         cfg = self.cfg
         T = h.shape[0]
         hn, rstd = fused.rmsnorm_fwd(h, self.w("final_norm"), cfg.norm_eps)
@@ -422,12 +431,11 @@ class LlamaModel(nn.Module):
         gW = self.g("lm_head.weight")
         dhn = torch.empty_like(hn) if want_grad else None
         loss_sum = torch.zeros((), device=h.device, dtype=torch.float32)
-        tflat = targets.reshape(-1)
         step = self.head_chunk_tokens
         for t0 in range(0, T, step):
             t1 = min(T, t0 + step)
             logits = gemm(hn[t0:t1], W)
-            losses = fused.cross_entropy_fwd_bwd_(logits, tflat[t0:t1], loss_weight)
+            losses = chunk_loss(logits, t0, t1)
             loss_sum += losses.sum()
             if want_grad:
                 gemm(logits, W, trans_b=True, out=dhn[t0:t1])
@@ -458,6 +466,34 @@ class LlamaModel(nn.Module):
         ring = self._ring(ring, S)
         if loss_weight is None:
             loss_weight = 1.0 / (B * S * ring.degree)
+        return self._forward_backward(tokens, self._cross_entropy_head(targets, loss_weight), loss_weight, ring)
+
+    def forward_backward_distill(self, tokens: torch.Tensor, teacher_logprobs: torch.Tensor, teacher_ids: torch.Tensor,
+                                 loss_weight: Optional[float] = None, ring: Optional[RingContext] = None, *,
+                                 temperature: float = 1.0, tail: str = "renormalize") -> torch.Tensor:
+        """``forward_backward`` with the divergence from a teacher in place of the cross-entropy.
+
+        teacher_logprobs / teacher_ids: [B, S_local, K], what ``token_logprobs(top_k=K, temperature=temperature)`` of the
+        teacher gave for the same positions (entries of -1 are absent, positions without entries are left out). See
+        ``ops.logprobs.distill_topk`` for the loss and ``tail``. ``loss_weight`` also carries a factor of temperature^2
+        where one is wanted."""
+        B, S = tokens.shape
+        ring = self._ring(ring, S)
+        if loss_weight is None:
+            loss_weight = 1.0 / (B * S * ring.degree)
+        K = teacher_ids.shape[-1]
+        if tuple(teacher_ids.shape[:-1]) != (B, S) or teacher_logprobs.shape != teacher_ids.shape:
+            raise ValueError(f"teacher tensors have shapes {tuple(teacher_logprobs.shape)} and {tuple(teacher_ids.shape)}, "
+                             f"expected ({B}, {S}, K)")
+        values, ids = teacher_logprobs.reshape(B * S, K), teacher_ids.reshape(B * S, K)
+
+        def head(logits, t0, t1):
+            return distill_topk_fwd_bwd_(logits, values[t0:t1], ids[t0:t1], loss_weight, temperature=temperature, tail=tail)
+
+        return self._forward_backward(tokens, head, loss_weight, ring)
+
+    def _forward_backward(self, tokens: torch.Tensor, head: Callable, loss_weight: float, ring: RingContext) -> torch.Tensor:
+        B, S = tokens.shape
         with torch.no_grad():
             with trace_range("embedding"):
                 h = fused.embedding_fwd(tokens, self.w("embed.weight"))
@@ -469,7 +505,7 @@ class LlamaModel(nn.Module):
             if "gu@host" in self.remat.saved and h.is_cuda:
                 self._start_fetch_gu(self.cfg.n_layers - 1)   # under the LM head instead of in front of the last layer
             with trace_range("head+loss"):
-                loss, dh = self._head_loss(h, targets, loss_weight, want_grad=True)
+                loss, dh = self._head_loss(h, head, loss_weight, want_grad=True)
             del h
             for l in reversed(range(self.cfg.n_layers)):
                 with trace_range(f"layer{l}.backward"):
@@ -494,6 +530,26 @@ class LlamaModel(nn.Module):
         B, S, H = hn.shape
         return gemm(hn.view(B * S, H), self.w("lm_head.weight")).view(B, S, -1)
 
+    def token_logprobs(self, tokens: torch.Tensor, targets: Optional[torch.Tensor] = None, *, top_k: int = 0,
+                       temperature: float = 1.0, ignore_index: int = -100,
+                       ring: Optional[RingContext] = None) -> TokenLogprobs:
+        """Log-probabilities of ``targets`` [B, S_local] (the tokens that the positions predict), the entropies, and the
+        ``top_k`` most likely tokens (no gradient tracking). The full logits never exist: the head runs over chunks of
+        ``head_chunk_tokens``. See ``ops.logprobs.token_logprobs``."""
+        B, S = tokens.shape
+        hn = self.forward(tokens, ring).view(B * S, -1)
+        if targets is not None and targets.shape != tokens.shape:
+            raise ValueError(f"targets have shape {tuple(targets.shape)}, the tokens {tuple(tokens.shape)}")
+        tflat = targets.reshape(-1) if targets is not None else None
+        W = self.w("lm_head.weight")
+        parts = []
+        with torch.no_grad():
+            for t0 in range(0, B * S, self.head_chunk_tokens):
+                t1 = min(B * S, t0 + self.head_chunk_tokens)
+                parts.append(token_logprobs(gemm(hn[t0:t1], W), tflat[t0:t1] if tflat is not None else None, top_k=top_k,
+                                            temperature=temperature, ignore_index=ignore_index))
+        return TokenLogprobs(*(torch.cat(p).view(B, S, *p[0].shape[1:]) if p[0] is not None else None for p in zip(*parts)))
+
     def loss(self, tokens: torch.Tensor, targets: torch.Tensor, ring: Optional[RingContext] = None) -> torch.Tensor:
         """Mean token cross-entropy as an autograd scalar: ``model.loss(x, y).backward()`` adds the
         gradients into the flat fp32 buffer (``param.main_grad``) like forward_backward does."""
@@ -515,7 +571,7 @@ class _LlamaLossFn(torch.autograd.Function):
             h, saved = model._layer_forward(l, h, B, S, ring, keep=True)
             saved_all.append(saved)
         # the head computes its own backward in the same sweep; dh is scaled by grad_out in backward()
-        loss, dh = model._head_loss(h, targets, loss_weight, want_grad=True)
+        loss, dh = model._head_loss(h, model._cross_entropy_head(targets, loss_weight), loss_weight, want_grad=True)
         ctx.model, ctx.saved_all, ctx.dh, ctx.meta = model, saved_all, dh, (B, S, ring, tokens)
         return loss
 

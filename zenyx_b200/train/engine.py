@@ -131,11 +131,27 @@ class LlamaEngine:
         device scalar; summing it over ranks gives the global mean token loss)."""
         if not presharded:
             tokens, targets = self.shard_batch(tokens), self.shard_batch(targets)
-        loss_weight = 1.0 / (self.cfg.global_batch * self.cfg.seq_len)
         ring = self.ring
+        return self._step(tokens, lr, lambda i, weight: self.model.forward_backward(
+            tokens[i: i + 1], targets[i: i + 1], weight, ring))
+
+    def distill_step(self, tokens: torch.Tensor, teacher_logprobs: torch.Tensor, teacher_ids: torch.Tensor,
+                     lr: Optional[float] = None, presharded: bool = False, *, temperature: float = 1.0,
+                     tail: str = "renormalize") -> torch.Tensor:
+        """``train_step`` on what a teacher wrote down for the same tokens ([global_batch, seq_len, K] each, see
+        ``LlamaModel.forward_backward_distill``)."""
+        if not presharded:
+            tokens = self.shard_batch(tokens)
+            teacher_logprobs, teacher_ids = self.shard_batch(teacher_logprobs), self.shard_batch(teacher_ids)
+        ring = self.ring
+        return self._step(tokens, lr, lambda i, weight: self.model.forward_backward_distill(
+            tokens[i: i + 1], teacher_logprobs[i: i + 1], teacher_ids[i: i + 1], weight, ring, temperature=temperature, tail=tail))
+
+    def _step(self, tokens: torch.Tensor, lr: Optional[float], micro_batch) -> torch.Tensor:
+        loss_weight = 1.0 / (self.cfg.global_batch * self.cfg.seq_len)
         loss = torch.zeros((), device=self.ctx.device, dtype=torch.float32)
         for i in range(tokens.shape[0]):
-            loss += self.model.forward_backward(tokens[i: i + 1], targets[i: i + 1], loss_weight, ring)
+            loss += micro_batch(i, loss_weight)
         timed = tokens.is_cuda
         if timed:   # two event records per step; read through optimizer_step_ms() once the step has finished
             if self._opt_events is None:

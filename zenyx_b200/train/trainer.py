@@ -91,17 +91,7 @@ class Trainer:
 
     def train_step(self, batch: torch.Tensor, target: torch.Tensor, criterion: Optional[nn.Module] = None) -> float:
         if self.engine is not None:
-            cur = self.config.curriculum
-            if cur is not None:
-                self.engine.set_ring_degree(cur.degree_at(self.step))
-            local = self.engine.train_step(batch, target, lr=self._lr())
-            loss = self.engine.global_loss(local)       # reads the loss back: the step's kernels have finished
-            self._raise_on_kernel_error()
-            if cur is not None:
-                cur.step(loss)
-            self.step += 1
-            self.memory.snapshot()
-            return loss
+            return self._engine_step(lambda: self.engine.train_step(batch, target, lr=self._lr()))
         if criterion is None:
             raise ValueError("the generic path needs a criterion: train_step(batch, target, criterion)")
         self.model.train()
@@ -135,6 +125,28 @@ class Trainer:
         self.step += 1
         self.memory.snapshot()
         return float(reduced.item() / get_world_size())
+
+    def distill_step(self, tokens: torch.Tensor, teacher_logprobs: torch.Tensor, teacher_ids: torch.Tensor, *,
+                     temperature: float = 1.0, tail: str = "renormalize") -> float:
+        """One optimizer step of the flagship on what a teacher wrote down for the same tokens: ``teacher_logprobs`` and
+        ``teacher_ids`` [global_batch, seq_len, K] from ``LlamaModel.token_logprobs(top_k=K)``. Returns the global mean
+        divergence. What the loss is: ``ops.logprobs.distill_topk``."""
+        if self.engine is None:
+            raise ValueError("distill_step needs the flagship path: Trainer(LlamaConfig, ...)")
+        return self._engine_step(lambda: self.engine.distill_step(tokens, teacher_logprobs, teacher_ids, lr=self._lr(),
+                                                                  temperature=temperature, tail=tail))
+
+    def _engine_step(self, step: Callable[[], torch.Tensor]) -> float:
+        cur = self.config.curriculum
+        if cur is not None:
+            self.engine.set_ring_degree(cur.degree_at(self.step))
+        loss = self.engine.global_loss(step())          # reads the loss back: the step's kernels have finished
+        self._raise_on_kernel_error()
+        if cur is not None:
+            cur.step(loss)
+        self.step += 1
+        self.memory.snapshot()
+        return loss
 
     def _raise_on_kernel_error(self) -> None:
         """Reads the device status word that the kernels' bounded waits write when they give up (a peer

@@ -4,6 +4,7 @@
 //   bucket:      q = exp(v), q_r = max(0, 1 - sum q), p_r = the sum of p outside the columns;   + q_r (log q_r - log p_r)
 //   temperature dloss/dx_j = p_j - q_j  (bucket, outside the columns: p_j (1 - q_r / p_r))
 // Bound by the bytes of the logits, read once, and of the gradient.
+#include <algorithm>
 #include <type_traits>
 #include "rows.cuh"
 
@@ -714,13 +715,32 @@ __global__ void __launch_bounds__(kThreads, 4) distill_bwd_kernel(DistillArgs a,
 // ------------------------------------------------------------------------------------------
 // Launches
 // ------------------------------------------------------------------------------------------
+// Blocks a row. What counts is how many bytes of slices an SM holds, and then how few blocks they are in (each has its
+// fixed work): the largest sum over four to six blocks, fewer blocks unless more hold a sixteenth more. 4096 x 128256 bf16: six blocks a row (five slices of 43 KB on an
+// SM) 392 us, five 403, four and eight (192 KB held) 437 and 433; 4000 x 50257: two (four of 50 KB) 163, three (six of
+// 34 KB) 181, one (two of 100 KB) 192, four (six of 25 KB) 196; 4096 x 32000 fp32: three 170, two and four 173.
+// Five and seven are left out: seven measured 262 us where six took 243 (2048 x 151936), five never was the best.
+// Few rows are split further, as long as the grid stays below five blocks an SM and a worker has a vector: 150 x 50257 takes
+// 15.3 us with four blocks a row, 16.3 with two, 19.1 with eight.
+int blocks_a_row(int vecs, int rows, int sm_count) {
+  constexpr int kSizes[] = {1, 2, 3, 4, 6, 8};
+  constexpr int kSmemOfSm = 228 * 1024, kOverhead = 1024 + (int)sizeof(DistillShared);
+  int best = kMaxCluster, held = 0;
+  for (int c : kSizes) {
+    const int slice = (vecs + c - 1) / c * 16, n = std::min(6, kSmemOfSm / (slice + kOverhead));
+    if (n >= 4 && n * slice > held + held / 16) {
+      best = c;
+      held = n * slice;
+    }
+  }
+  for (int c : kSizes)
+    if (c > best && (int64_t)rows * c <= 5 * sm_count && vecs / c >= kWorkers) best = c;
+  return best;
+}
 template <class T, bool WRITE>
 void launch_distill(const DistillArgs& a) {
   const int vecs = most_vecs<T>(a.logits, a.ld, a.rows, a.V);
-  // Blocks a row: slices of at most 32 KB, six of which fit an SM; smaller ones for few rows.
-  int cluster = 1;
-  while (cluster < kMaxCluster && vecs > cluster * 2048 + 64) cluster *= 2;
-  while (cluster < kMaxCluster && (int64_t)a.rows * cluster * 2 <= 4 * a.sm_count && vecs / (cluster * 2) >= kWorkers) cluster *= 2;
+  const int cluster = blocks_a_row(vecs, a.rows, a.sm_count);
   const int smem = (vecs + cluster - 1) / cluster * 16;
   launch(distill_kernel<T, WRITE>, a.rows, cluster, true, kWorkers + 32, smem, a.stream, a, cluster);
 }

@@ -267,8 +267,12 @@ __device__ __forceinline__ void distill_auxiliary(const DistillArgs& a, DistillS
     const Row<T> row(a.logits, r, a.ld, a.V);
     const int per = (row.vecs + cluster - 1) / cluster;
     const int v0 = min(rank * per, row.vecs), v1 = min(v0 + per, row.vecs);
-    if (n >= 1 && !mbar_wait_w(&sh.empty, (n - 1) & 1, &sh.abort)) return leave(kSiteEmpty);
     const int w0 = max(v0, row.first_full), w1 = min(v1, row.end_full);
+    if (n >= 1) {
+      // the workers still have the slice: into the L2 cache with the next one meanwhile
+      if (lane == 0 && t.live && w1 > w0) prefetch_l2(row.at(w0), (uint32_t)(w1 - w0) * 16);
+      if (!mbar_wait_w(&sh.empty, (n - 1) & 1, &sh.abort)) return leave(kSiteEmpty);
+    }
     if (lane == 0) {
       if (t.live && w1 > w0) {
         fence_proxy_async_smem();     // the stage was written by threads before

@@ -324,6 +324,11 @@ __device__ __forceinline__ void store_to_cta(void* p, uint32_t rank, uint64_t v)
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(map_to_cta(p, rank)), "l"(v) : "memory");
 }
 
+// bytes: whole 16-byte vectors of one row.
+__device__ __forceinline__ void prefetch_l2(const uint4* p, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
+
 // ------------------------------------------------------------------------------------------
 // Launches
 // ------------------------------------------------------------------------------------------

@@ -358,8 +358,9 @@ void launch(void (*kernel)(P...), int rows, int blocks_a_row, bool cluster, int 
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster && blocks_a_row > 1 ? 1 : 0;
-  // the limit is raised, never lowered: launches of other sizes rely on it
-  if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+  // 48 KB go without asking, the kernel's own arrays included. The limit is raised, never lowered: launches of other sizes
+  // rely on it.
+  if (smem > 32 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
   cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 

@@ -534,3 +534,20 @@ def test_logits_overwritten_before_the_backward_are_noticed():
     distill_topk_fwd_bwd_(z.detach(), torch.zeros(4, 1, device="cuda"), y[:, None], 1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         out.logprobs.sum().backward()
+
+
+@pytest.mark.parametrize("V", [15000, 20000, 22800, 23100, 23500, 24000, 24570, 25000, 26000, 27000, 28000, 33000, 47000])
+def test_vocabularies_around_the_sizes_of_shared_memory(V):
+    x, y, gen = _logits(800, V, torch.bfloat16, seed=V)
+    values, ids = _teacher(x, 5, gen)
+    out = torch.empty_like(x)
+    loss = distill_topk_fwd_bwd_(x, values, ids, 1.0, out=out)
+    few = slice(797, 800)
+    ref, grad, off, grad_off = oracle.distill(x[few], values[few], ids[few], 1.0, "renormalize")
+    oracle.check(loss[few], ref, off, "loss")
+    oracle.check(out[few], grad, grad_off, "gradient")
+    for dtype, K in ((torch.bfloat16, 3), (torch.float32, 128)):
+        _check_fwd(x[:200].to(dtype), y[:200], K)
+    del x, out
+    x, y, _ = _logits(3, 5 * V, torch.bfloat16, seed=V)
+    _check_fwd(x, y, 9)

@@ -265,7 +265,7 @@ struct FwdShared {
   float cta[kMaxCluster][3];
   float m;
   double log_l;
-  uint32_t least[kWarps], most[kWarps];
+  uint32_t least[4][kWarps], most[kWarps];
 };
 
 // One group of vectors into the running sums (l and s as pairs).
@@ -406,11 +406,14 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(LogprobsArgs 
   t = warp_join(t, c2);
   if (lane == 0) sh.part[warp] = t;
   if (TOP) {
-    const int q = (K + warps - 1) / warps;        // a warp has that many threads?
     const uint32_t sorted = warp_sort(own);
-    const uint32_t least = __shfl_sync(0xffffffffu, sorted, min(q, 32) - 1);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {       // what ceil(K / 2^j) of the warp's threads reach
+      const int q = (K + (1 << j) - 1) >> j;
+      const uint32_t least = __shfl_sync(0xffffffffu, sorted, min(q, 32) - 1);
+      if (lane == 0) sh.least[j][warp] = q <= 32 ? least : 0;
+    }
     if (lane == 0) {
-      sh.least[warp] = q <= 32 ? least : 0;
       sh.most[warp] = order_key(t.m);
     }
     if (tid == 0) top.n = top.groups = 0;
@@ -444,10 +447,20 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(LogprobsArgs 
   if (!TOP && warp == warps - 1) join();
   if (TOP) {
     bool joined = false;
-    uint32_t lo = sh.least[0], hi = sh.most[0];
-    for (int w = 1; w < warps; ++w) {
-      lo = min(lo, sh.least[w]);
-      hi = max(hi, sh.most[w]);
+    // 2^j warps of which each has ceil(K / 2^j) threads: the 2^j-th largest over the warps, the best over j
+    uint32_t lo, hi;
+    {
+      static_assert(kWarps == 8, "a lane for each warp and j");
+      const int w = lane & 7, j = lane >> 3;
+      const uint32_t mine = w < warps ? sh.least[j][w] : 0;
+      int above = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t other = __shfl_sync(0xffffffffu, mine, (lane & 24) | i);
+        above += other > mine || (other == mine && i < w);
+      }
+      lo = __reduce_max_sync(0xffffffffu, above == (1 << j) - 1 ? mine : 0);
+      hi = __reduce_max_sync(0xffffffffu, w < warps ? sh.most[w] : 0);
     }
     int n = 0;
     if (!is_bad(key_value(hi)) && hi > kNegInfKey) {   // else this block has no alternatives

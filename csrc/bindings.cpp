@@ -559,7 +559,7 @@ zx::IdArray id_array(const Tensor& t, int64_t n, const Tensor& like, const char*
   return a;
 }
 zx::LogprobsArgs logprobs_args(const Tensor& logits, const c10::optional<Tensor>& targets, const Tensor& entropy,
-                               const Tensor& stats, double temperature) {
+                               const c10::optional<Tensor>& stats, double temperature) {
   zx::LogprobsArgs a;
   a.type = logit_type(logits, "logits");
   check_logits(logits);
@@ -571,14 +571,14 @@ zx::LogprobsArgs logprobs_args(const Tensor& logits, const c10::optional<Tensor>
   a.temperature = (float)temperature;
   if (targets.has_value()) a.targets = id_array(*targets, a.rows, logits, "targets");
   a.entropy = float_rows(entropy, a.rows, logits, "entropy");
-  a.stats = float_rows(stats, 2 * (int64_t)a.rows, logits, "stats");
+  a.stats = const_cast<float*>(float_rows(stats, 2 * (int64_t)a.rows, logits, "stats"));
   return a;
 }
 
 // Per row of logits: log-probability of targets (int; outside [0, V): the row is left out), entropy, (maximum, sum of
-// exponentials) in stats, and the top_ids.size(1) most likely columns with their log-probabilities.
+// exponentials) in stats, which may be absent, and the top_ids.size(1) most likely columns with their log-probabilities.
 void token_logprobs_fwd(const Tensor& logits, const c10::optional<Tensor>& targets, const c10::optional<Tensor>& logprobs,
-                        Tensor& entropy, Tensor& stats, const c10::optional<Tensor>& top_logprobs,
+                        Tensor& entropy, const c10::optional<Tensor>& stats, const c10::optional<Tensor>& top_logprobs,
                         const c10::optional<Tensor>& top_ids, double temperature) {
   zx::LogprobsArgs a = logprobs_args(logits, targets, entropy, stats, temperature);
   TORCH_CHECK(targets.has_value() == logprobs.has_value(), "targets and logprobs come together");
@@ -673,7 +673,38 @@ void distill_topk(const Tensor& logits, const Tensor& values, const Tensor& ids,
   check_launch("distill_topk");
 }
 
-// ---- the same as autograd functions (in C++: a step of a small model is mostly host time) ----
+// ---- the same as users call them, with their checks and as autograd functions. In C++: a call for a few rows is mostly
+// host time. The Python forms in ops/logprobs.py check the same for CPU tensors. ----
+
+void check_user_logits(const Tensor& x, double temperature) {
+  TORCH_CHECK_TYPE(x.scalar_type() == torch::kBFloat16 || x.scalar_type() == torch::kFloat16 || x.scalar_type() == torch::kFloat32,
+                   "logits are bf16, fp16 or fp32, not ", x.scalar_type());
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= zx::kHeadMaxVocab, "logits are [..., V] with 1 <= V <= ",
+                    zx::kHeadMaxVocab, ", not ", x.sizes());
+  TORCH_CHECK_VALUE(temperature >= 1e-4 && temperature <= 1e4, "the temperature lies in [0.0001, 10000], not ", temperature);
+}
+// ids [..., K] (K > 0) or [...] for logits [..., V]
+void check_user_ids(const char* name, const Tensor& ids, int64_t K, const Tensor& logits) {
+  TORCH_CHECK_TYPE(ids.scalar_type() == torch::kInt64 || ids.scalar_type() == torch::kInt32, name, " are int64 or int32, not ",
+                   ids.scalar_type());
+  const auto lead = logits.sizes().slice(0, logits.dim() - 1);
+  const bool shaped = ids.dim() == (int64_t)lead.size() + (K > 0 ? 1 : 0) && ids.sizes().slice(0, lead.size()) == lead &&
+                      (K == 0 || ids.size(-1) == K);
+  TORCH_CHECK_VALUE(shaped, name, " have shape ", ids.sizes(), ", expected ", lead, K > 0 ? " and their number" : "");
+  TORCH_CHECK_VALUE(ids.device() == logits.device(), name, " are on ", ids.device(), ", the logits on ", logits.device());
+}
+void check_teacher(const Tensor& logits, const Tensor& values, const Tensor& ids, const std::string& tail) {
+  TORCH_CHECK_VALUE(tail == "renormalize" || tail == "bucket", "tail is 'renormalize' or 'bucket', not '", tail, "'");
+  const int64_t K = ids.dim() > 0 ? ids.size(-1) : 0;
+  TORCH_CHECK_VALUE(K >= 1 && K <= zx::kHeadMaxTop, "teacher_ids are [..., K] with 1 <= K <= ", zx::kHeadMaxTop, ", not ", ids.sizes());
+  check_user_ids("teacher_ids", ids, K, logits);
+  const auto t = values.scalar_type();
+  TORCH_CHECK_TYPE(t == torch::kBFloat16 || t == torch::kFloat16 || t == torch::kFloat32,
+                   "teacher_logprobs are bf16, fp16 or fp32, not ", t);
+  TORCH_CHECK_VALUE(values.sizes() == ids.sizes(), "teacher_logprobs have shape ", values.sizes(), ", teacher_ids ", ids.sizes());
+  TORCH_CHECK_VALUE(values.device() == logits.device(), "teacher_logprobs are on ", values.device(), ", the logits on ", logits.device());
+  TORCH_CHECK_VALUE(!values.requires_grad() || !at::GradMode::is_enabled(), "the teacher gets no gradient: detach teacher_logprobs");
+}
 
 // Gradients that have none of their own: an error when somebody asks for it, as torch.autograd's once_differentiable.
 Tensor differentiable_once(const Tensor& g) {
@@ -695,33 +726,43 @@ std::vector<int64_t> lead_of(const Tensor& logits) {
   return s;
 }
 
+struct Scored {
+  Tensor logprobs, entropy, stats, top, ids;    // undefined: not asked for
+};
+Scored score(const Tensor& logits, const Tensor& targets, int64_t top_k, double temperature, bool with_stats) {
+  const Tensor x = rows_of(logits);
+  auto lead = lead_of(logits);
+  const auto f32 = at::TensorOptions().dtype(torch::kFloat32).device(x.device());
+  Scored o;
+  o.entropy = at::empty(lead, f32);
+  if (targets.defined()) o.logprobs = at::empty(lead, f32);
+  if (with_stats) o.stats = at::empty({x.size(0), 2}, f32);
+  if (top_k > 0) {
+    lead.push_back(top_k);
+    o.top = at::empty(lead, f32);
+    o.ids = at::empty(lead, f32.dtype(torch::kInt64));
+  }
+  auto opt = [](const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; };
+  auto flat = [&](const Tensor& t) {
+    return t.defined() ? c10::optional<Tensor>(t.dim() == 2 ? t : t.view({x.size(0), top_k})) : c10::nullopt;
+  };
+  token_logprobs_fwd(x, opt(targets), opt(o.logprobs), o.entropy, opt(o.stats), flat(o.top), flat(o.ids), temperature);
+  return o;
+}
+
 struct TokenLogprobsFn : public torch::autograd::Function<TokenLogprobsFn> {
-  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits,
-                                                const c10::optional<Tensor>& targets, int64_t top_k, double temperature) {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits, const Tensor& y,
+                                                int64_t top_k, double temperature) {
     at::AutoDispatchBelowADInplaceOrView below;
-    const Tensor x = rows_of(logits);
-    auto lead = lead_of(logits);
-    const auto f32 = x.options().dtype(torch::kFloat32);
-    const bool with_y = targets.has_value();
-    const Tensor y = with_y ? targets->contiguous() : Tensor();
-    Tensor entropy = at::empty(lead, f32), stats = at::empty({x.size(0), 2}, f32), lp, top, ids;
-    if (with_y) lp = at::empty(lead, f32);
+    const Scored o = score(logits, y, top_k, temperature, true);
+    torch::autograd::variable_list out{o.entropy};
+    if (y.defined()) out.push_back(o.logprobs);
     if (top_k > 0) {
-      lead.push_back(top_k);
-      top = at::empty(lead, f32);
-      ids = at::empty(lead, x.options().dtype(torch::kInt64));
+      out.push_back(o.top);
+      out.push_back(o.ids);
+      ctx->mark_non_differentiable({o.ids});
     }
-    auto opt = [](const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; };
-    auto flat = [&](const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t.view({x.size(0), top_k})) : c10::nullopt; };
-    token_logprobs_fwd(x, opt(y), opt(lp), entropy, stats, flat(top), flat(ids), temperature);
-    torch::autograd::variable_list out{entropy};
-    if (with_y) out.push_back(lp);
-    if (top_k > 0) {
-      out.push_back(top);
-      out.push_back(ids);
-      ctx->mark_non_differentiable({ids});
-    }
-    ctx->save_for_backward({logits, y, entropy, ids, stats});
+    ctx->save_for_backward({logits, y, o.entropy, o.ids, o.stats});
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["top_k"] = top_k;
     ctx->set_materialize_grads(false);
@@ -749,11 +790,25 @@ struct TokenLogprobsFn : public torch::autograd::Function<TokenLogprobsFn> {
 using MaybeTensor = c10::optional<Tensor>;
 // (logprobs, entropy, top_logprobs, top_ids) of logits [..., V]
 std::tuple<MaybeTensor, Tensor, MaybeTensor, MaybeTensor> token_logprobs(const Tensor& logits, const MaybeTensor& targets, int64_t top_k,
-                                                                         double temperature) {
-  const auto out = TokenLogprobsFn::apply(logits, targets, top_k, temperature);
+                                                                         double temperature, int64_t ignore_index) {
+  check_user_logits(logits, temperature);
+  const int64_t V = logits.size(-1), most = std::min<int64_t>(V, zx::kHeadMaxTop);
+  TORCH_CHECK_VALUE(top_k >= 0 && top_k <= most, "top_k lies in [0, ", most, "], not ", top_k);
+  TORCH_CHECK_VALUE(ignore_index < 0 || ignore_index >= V, "ignore_index ", ignore_index, " is a token");
+  Tensor y;
+  if (targets.has_value()) {
+    check_user_ids("targets", *targets, 0, logits);
+    y = targets->contiguous();
+  }
+  auto maybe = [](const Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); };
+  if (!at::GradMode::is_enabled() || !logits.requires_grad()) {
+    const Scored o = score(logits, y, top_k, temperature, false);
+    return {maybe(o.logprobs), o.entropy, maybe(o.top), maybe(o.ids)};
+  }
+  const auto out = TokenLogprobsFn::apply(logits, y, top_k, temperature);
   size_t i = 1;
   MaybeTensor lp, top, ids;
-  if (targets.has_value()) lp = out[i++];
+  if (y.defined()) lp = out[i++];
   if (top_k > 0) {
     top = out[i++];
     ids = out[i++];
@@ -789,8 +844,25 @@ struct DistillFn : public torch::autograd::Function<DistillFn> {
     return {differentiable_once(d), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
-Tensor distill_topk_loss(const Tensor& logits, const Tensor& values, const Tensor& ids, double temperature, bool bucket) {
-  return DistillFn::apply(logits, values, ids, temperature, bucket);
+Tensor distill_topk_loss(const Tensor& logits, const Tensor& values, const Tensor& ids, double temperature, const std::string& tail) {
+  check_user_logits(logits, temperature);
+  check_teacher(logits, values, ids, tail);
+  return DistillFn::apply(logits, values.detach(), ids, temperature, tail == "bucket");
+}
+// Losses [rows]; out, or the logits themselves, gets grad_scale times the gradient of their sum.
+Tensor distill_topk_fwd_bwd(const Tensor& logits, const Tensor& values, const Tensor& ids, double grad_scale, double temperature,
+                            const std::string& tail, const MaybeTensor& out) {
+  check_user_logits(logits, temperature);
+  TORCH_CHECK_VALUE(logits.dim() == 2 && (logits.size(1) == 1 || logits.stride(1) == 1), "logits are [rows, V] with contiguous columns");
+  check_teacher(logits, values, ids, tail);
+  const Tensor& d = out.has_value() ? *out : logits;
+  TORCH_CHECK_VALUE(d.sizes() == logits.sizes() && d.scalar_type() == logits.scalar_type() && d.device() == logits.device(),
+                    "out has the shape, type and device of the logits");
+  Tensor loss = at::empty({logits.size(0)}, at::TensorOptions().dtype(torch::kFloat32).device(logits.device()));
+  distill_topk(logits, values.contiguous(), ids.contiguous(), loss, c10::nullopt, c10::nullopt, d, grad_scale, temperature, tail == "bucket");
+  // a backward that has kept these logits is an error now instead of wrong
+  if (!d.is_inference()) d.unsafeGetTensorImpl()->bump_version();
+  return loss;
 }
 
 }  // namespace
@@ -821,6 +893,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("distill_topk", &distill_topk);
   m.def("token_logprobs", &token_logprobs);
   m.def("distill_topk_loss", &distill_topk_loss);
+  m.def("distill_topk_fwd_bwd", &distill_topk_fwd_bwd);
   m.def("kv_quant_e4m3", &kv_quant_e4m3);
   m.def("kv_dequant_e4m3", &kv_dequant_e4m3);
   m.def("adamw", &adamw);

@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(LogprobsArgs 
         if (tid == 0) {
           a.logprobs[r] = 0.f;
           a.entropy[r] = 0.f;
-          a.stats[(size_t)r * 2] = a.stats[(size_t)r * 2 + 1] = 0.f;
+          if (a.stats != nullptr) a.stats[(size_t)r * 2] = a.stats[(size_t)r * 2 + 1] = 0.f;
         }
         for (int k = tid; k < K; k += nt) {
           a.top_logprobs[(size_t)r * K + k] = -inf_f();
@@ -426,8 +426,10 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(LogprobsArgs 
     const double log_l = log((double)b.l);
     sh.m = b.m;
     sh.log_l = log_l;
-    a.stats[(size_t)r * 2] = b.m;
-    a.stats[(size_t)r * 2 + 1] = bad ? nan_f() : b.l;
+    if (a.stats != nullptr) {
+      a.stats[(size_t)r * 2] = b.m;
+      a.stats[(size_t)r * 2 + 1] = bad ? nan_f() : b.l;
+    }
     a.entropy[r] = bad ? nan_f() : (empty ? 0.f : (float)(log_l - kLn2 * (double)b.s / (double)b.l));
     if (y >= 0) a.logprobs[r] = bad ? nan_f() : (empty ? -inf_f() : (float)(kLn2 * rel2_exact(xy, b.m, c2) - log_l));
   };

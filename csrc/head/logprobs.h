@@ -30,7 +30,7 @@ struct LogprobsArgs {
   IdArray targets;             // [rows] or null: no row is left out, no log-probability of a token
   float* logprobs = nullptr;   // [rows] or null
   float* entropy = nullptr;    // [rows]
-  float* stats = nullptr;      // [rows, 2]: maximum and sum of the exponentials, written by the forward; 0 sum: no gradient
+  float* stats = nullptr;      // [rows, 2] or null in the forward: maximum and sum of the exponentials; 0 sum: no gradient
   int top_k = 0;
   float* top_logprobs = nullptr;   // [rows, top_k]
   int64_t* top_ids = nullptr;      // [rows, top_k]

@@ -551,3 +551,48 @@ def test_vocabularies_around_the_sizes_of_shared_memory(V):
     del x, out
     x, y, _ = _logits(3, 5 * V, torch.bfloat16, seed=V)
     _check_fwd(x, y, 9)
+
+
+def test_the_extension_refuses_what_the_cpu_form_does():
+    x, y, _ = _logits(3, 20, torch.float32)
+    ids, v = torch.zeros(3, 2, device="cuda", dtype=torch.int64), torch.zeros(3, 2, device="cuda")
+    for device in ("cpu", "cuda"):
+        x, y, ids, v = x.to(device), y.to(device), ids.to(device), v.to(device)
+        wide = torch.zeros(3, 129, device=device)
+        for error, bad in (
+                (ValueError, lambda: token_logprobs(x, y, top_k=21)), (ValueError, lambda: token_logprobs(x, y, top_k=-1)),
+                (ValueError, lambda: token_logprobs(x, y, temperature=0.0)),
+                (ValueError, lambda: token_logprobs(x, y, temperature=math.nan)),
+                (ValueError, lambda: token_logprobs(x, y, temperature=math.inf)),
+                (ValueError, lambda: token_logprobs(x, y, ignore_index=5)),
+                (ValueError, lambda: token_logprobs(wide.repeat(1, 2), top_k=129)),
+                (ValueError, lambda: token_logprobs(x, y[:2])), (ValueError, lambda: token_logprobs(x, y[:, None])),
+                (TypeError, lambda: token_logprobs(x, y.float())), (TypeError, lambda: token_logprobs(x.long(), y)),
+                (ValueError, lambda: token_logprobs(x[:, :0])), (ValueError, lambda: token_logprobs(x[0, 0])),
+                (ValueError, lambda: distill_topk(x, v, ids, tail="drop")), (ValueError, lambda: distill_topk(x, v[:, :1], ids)),
+                (ValueError, lambda: distill_topk(x, v[:2], ids[:2])), (ValueError, lambda: distill_topk(x, v, ids, temperature=-1.0)),
+                (ValueError, lambda: distill_topk(x, v[:, :0], ids[:, :0])), (ValueError, lambda: distill_topk(x, wide, wide.long())),
+                (ValueError, lambda: distill_topk(x, v.clone().requires_grad_(True), ids)),
+                (ValueError, lambda: distill_topk(x, v[0], ids[0])), (ValueError, lambda: distill_topk(x[0], v, ids)),
+                (TypeError, lambda: distill_topk(x, v, ids.float())), (TypeError, lambda: distill_topk(x, v.long(), ids)),
+                (ValueError, lambda: distill_topk_fwd_bwd_(x, v, ids, 1.0, out=torch.zeros(3, 21, device=device))),
+                (ValueError, lambda: distill_topk_fwd_bwd_(x, v, ids, 1.0, out=x.bfloat16())),
+                (ValueError, lambda: distill_topk_fwd_bwd_(x.t(), wide[:1, :2].expand(20, 2), torch.zeros(20, 2, device=device).long(), 1.0)),
+                (ValueError, lambda: distill_topk_fwd_bwd_(x[None], v[None], ids[None], 1.0)),
+                (ValueError, lambda: distill_topk_fwd_bwd_(x, v, ids, 1.0, temperature=1e5)),
+                (ValueError, lambda: distill_topk_fwd_bwd_(x, v, ids, 1.0, tail="")),
+                (ValueError, lambda: distill_topk_fwd_bwd_(x, v, ids[:, :1], 1.0))):
+            with pytest.raises(error):
+                bad()
+
+
+def test_scoring_without_gradients_is_scoring_with_them():
+    x, y, _ = _logits(5, 1000, torch.bfloat16)
+    y[3] = -100
+    with_grad = token_logprobs(x.clone().requires_grad_(True), y, top_k=4)
+    with torch.inference_mode():
+        z = x.clone()
+        without = token_logprobs(z, y, top_k=4)
+        distill_topk_fwd_bwd_(z, without.top_logprobs, without.top_ids, 1.0)
+    for a, b in zip(with_grad, without):
+        assert torch.equal(a, b)

@@ -71,12 +71,6 @@ def _rows(logits: torch.Tensor) -> torch.Tensor:
     return x if x.shape[1] == 1 or x.stride(1) == 1 else x.contiguous()
 
 
-def _overwritten(x: torch.Tensor) -> None:
-    """Tells autograd, so that a backward that has kept these logits is an error instead of wrong."""
-    if not x.is_inference():
-        torch.autograd.graph.increment_version(x)
-
-
 def _wide(x: torch.Tensor) -> torch.Tensor:
     return x if x.dtype == torch.float64 else x.float()
 
@@ -143,7 +137,8 @@ def token_logprobs_bwd(logits: torch.Tensor, targets: Optional[torch.Tensor], ou
 
         _ext.C().token_logprobs_bwd(logits, targets.contiguous() if targets is not None else None, out.entropy, stats,
                                     out.top_ids, fp32(d_logprobs), fp32(d_entropy), fp32(d_top), d_logits, temperature)
-        _overwritten(d_logits)
+        if not d_logits.is_inference():     # a backward that has kept these logits is an error now instead of wrong
+            torch.autograd.graph.increment_version(d_logits)
         return d_logits
     x = _wide(logits)
     m, l = stats[:, 0], stats[:, 1]
@@ -198,6 +193,8 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     log-probabilities. Rows whose target is ``ignore_index`` (or any other number outside [0, V)) are left out;
     without targets every row counts and ``logprobs`` is None.
     """
+    if logits.is_cuda:      # the extension checks the same
+        return TokenLogprobs(*_ext.C().token_logprobs(logits, targets, top_k, temperature, ignore_index))
     _check_logits(logits, temperature)
     V, shape = logits.shape[-1], logits.shape[:-1]
     if not 0 <= top_k <= min(V, MAX_TOP):
@@ -206,8 +203,6 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
         raise ValueError(f"ignore_index {ignore_index} is a token")
     if targets is not None:
         _check_ids("targets", targets, shape, logits)
-    if logits.is_cuda:
-        return TokenLogprobs(*_ext.C().token_logprobs(logits, targets, top_k, temperature))
     if targets is not None:
         targets = targets.reshape(-1)
     lp, entropy, top, ids = _TokenLogprobsFn.apply(_rows(logits), targets, int(top_k), float(temperature))
@@ -275,6 +270,8 @@ def distill_topk_fwd_bwd_(logits: torch.Tensor, teacher_logprobs: torch.Tensor, 
                           out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Overwrites `logits` [rows, V] (or fills `out`, which leaves them alone) with grad_scale * d(sum of
     losses)/d(logits); returns the per-row losses (fp32). What the losses are: see ``distill_topk``."""
+    if logits.is_cuda:      # the extension checks the same
+        return _ext.C().distill_topk_fwd_bwd(logits, teacher_logprobs, teacher_ids, grad_scale, temperature, tail, out)
     _check_logits(logits, temperature)
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("logits are [rows, V] with contiguous columns")
@@ -282,12 +279,6 @@ def distill_topk_fwd_bwd_(logits: torch.Tensor, teacher_logprobs: torch.Tensor, 
     out = logits if out is None else out
     if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
         raise ValueError("out has the shape, type and device of the logits")
-    if logits.is_cuda and _ext.use_cuda_kernels(logits):
-        loss = torch.empty(logits.shape[0], device=logits.device, dtype=torch.float32)
-        _ext.C().distill_topk(logits, teacher_logprobs.contiguous(), teacher_ids.contiguous(), loss, None, None, out,
-                              grad_scale, temperature, tail == "bucket")
-        _overwritten(out)
-        return loss
     loss, grad = _distill_torch(_wide(logits), teacher_logprobs, teacher_ids, temperature, tail == "bucket")
     out.copy_(grad * grad_scale)
     return loss
@@ -326,10 +317,10 @@ def distill_topk(logits: torch.Tensor, teacher_logprobs: torch.Tensor, teacher_i
     the sum of both. The loss is infinite where the student's logit of a token with q > 0 is -inf. Softened
     targets are usually weighted with temperature^2: that is left to the caller.
     """
+    if logits.is_cuda:      # the extension checks the same
+        return _ext.C().distill_topk_loss(logits, teacher_logprobs, teacher_ids, temperature, tail)
     _check_logits(logits, temperature)
     _check_teacher(logits, teacher_logprobs, teacher_ids, tail)
-    if logits.is_cuda:
-        return _ext.C().distill_topk_loss(logits, teacher_logprobs.detach(), teacher_ids, temperature, tail == "bucket")
     K = teacher_ids.shape[-1]
     loss = _DistillFn.apply(_rows(logits), teacher_logprobs.detach().reshape(-1, K), teacher_ids.reshape(-1, K),
                             float(temperature), tail == "bucket")

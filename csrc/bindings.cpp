@@ -751,9 +751,10 @@ Scored score(const Tensor& logits, const Tensor& targets, int64_t top_k, double 
 }
 
 struct TokenLogprobsFn : public torch::autograd::Function<TokenLogprobsFn> {
-  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits, const Tensor& y,
-                                                int64_t top_k, double temperature) {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits,
+                                                const c10::optional<Tensor>& targets, int64_t top_k, double temperature) {
     at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor y = targets.value_or(Tensor());
     const Scored o = score(logits, y, top_k, temperature, true);
     torch::autograd::variable_list out{o.entropy};
     if (y.defined()) out.push_back(o.logprobs);
@@ -805,7 +806,7 @@ std::tuple<MaybeTensor, Tensor, MaybeTensor, MaybeTensor> token_logprobs(const T
     const Scored o = score(logits, y, top_k, temperature, false);
     return {maybe(o.logprobs), o.entropy, maybe(o.top), maybe(o.ids)};
   }
-  const auto out = TokenLogprobsFn::apply(logits, y, top_k, temperature);
+  const auto out = TokenLogprobsFn::apply(logits, maybe(y), top_k, temperature);
   size_t i = 1;
   MaybeTensor lp, top, ids;
   if (y.defined()) lp = out[i++];

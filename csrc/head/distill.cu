@@ -3,7 +3,9 @@
 //   renormalize: q = softmax(v);                    loss = sum q_k (log q_k - log p_{i_k})
 //   bucket:      q = exp(v), q_r = max(0, 1 - sum q), p_r = the sum of p outside the columns;   + q_r (log q_r - log p_r)
 //   temperature dloss/dx_j = p_j - q_j  (bucket, outside the columns: p_j (1 - q_r / p_r))
-// Bound by the bytes of the logits, read once, and of the gradient.
+// Bound by the bytes of the logits, read once, and of the gradient. Measured on a B200 that copies 6557 GB/s, 64 of the
+// teacher's tokens: loss and gradient of 4096 x 128256 bf16 391 us (5.4 TB/s), 4096 x 32000 fp32 168 (6.2), 4000 x 50257
+// bf16 161 (5.0), 256 x 512 7.0 us; the loss alone of 4096 x 128256 227 us (4.6), its gradient from the statistics 317 (6.6).
 #include <algorithm>
 #include <type_traits>
 #include "rows.cuh"
@@ -118,9 +120,13 @@ __device__ __noinline__ void join_same(const Entries& e, int K, int* s_id, float
 // Loss (and gradient): the blocks of a cluster share a row, each with a slice of it in shared memory from the first look
 // to the gradient, so the logits are read once. The grid has a cluster for each row; one that is done with its row takes
 // the row of a cluster that has not started (cluster launch control), so that the blocks' barriers and the entries of the
-// next row are there when the slice is free. An auxiliary warp sees to that, starts the copy of the slice, takes the columns of the teacher's tokens out of it (-inf) when it is there, and weighs the next row's entries
-// meanwhile. Six blocks on an SM, at different points of their rows, keep the memory busy: a block's own chain (copy, sums,
-// exchange within the cluster, gradient) is several times the time in which the SM moves a slice.
+// next row are there when the slice is free. An auxiliary warp sees to that, starts the copy of the slice, takes the columns
+// of the teacher's tokens out of it (-inf) when it is there, and weighs the next row's entries meanwhile. Four to six blocks
+// on an SM, at different points of their rows, keep the memory busy: a block's own chain (copy, sums, exchange within the
+// cluster, gradient) is several times the time in which the SM moves a slice. What bounds it: 9.4 instructions a logit and
+// 2800 a block and row on the issue slots, and the shared memory that is filled. What it took the place of, 4096 x 128256:
+// the slice in registers 864 us, two stages a block 924, one grid of clusters without taking over rows 578, a ring between
+// warps that sum, write and copy 580, a row read again from the L2 cache by one block 441.
 //
 // The teacher's columns are kept apart so that the sum over all others is taken relative to their own maximum: the mass
 // outside keeps its digits when the teacher's tokens have nearly all of it.
@@ -633,7 +639,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 6) distill_kernel(DistillArgs a
 // ------------------------------------------------------------------------------------------
 // Gradient from the forward's statistics, one block a segment of a row. The first warps hold the teacher's entries.
 // ------------------------------------------------------------------------------------------
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;   // (128: 365 us instead of 317 for 4096 x 128256 bf16: the entries are a warp's work in each block)
 constexpr int kGradVecs = 8;    // vectors of a thread, all in flight
 
 template <class T>

@@ -13,7 +13,7 @@ namespace zx {
 enum LogitType : int { LOGIT_BF16 = 0, LOGIT_FP16 = 1, LOGIT_FP32 = 2 };
 
 constexpr int kHeadMaxTop = 128;          // most alternatives of a row
-constexpr int kHeadMaxVocab = 400000;     // most columns (a row of fp32 in the shared memory of eight blocks)
+constexpr int kHeadMaxVocab = 400000;     // most columns: a row of fp32 fits the shared memory of eight blocks, 200 KB each
 
 // Token numbers, 32 or 64 bits wide; what lies outside [0, V) is absent.
 struct IdArray {

@@ -158,6 +158,31 @@ def bench_fused(tokens=32768, H=4096, F=14336, Hq=32, Hkv=8, D=128):
     return out
 
 
+def bench_head(rows=4096, V=128256, K=64):
+    """The operators on one chunk of the 8B shape's logits: algorithmic bytes / time."""
+    from zenyx_b200.ops import _ext
+    from zenyx_b200.ops.logprobs import distill_topk_fwd_bwd_, token_logprobs, token_logprobs_bwd, token_logprobs_fwd
+
+    x = torch.randn(rows, V, device="cuda").bfloat16()
+    y = torch.randint(0, V, (rows,), device="cuda")
+    out, grad = token_logprobs(x, y, top_k=K), torch.empty_like(x)
+    scored, stats = token_logprobs_fwd(x, y, 0, 1.0)
+    g = torch.randn(rows, device="cuda")
+    recs = []
+    for name, passes, fn in (
+            ("token_logprobs", 1, lambda: token_logprobs(x, y)),
+            (f"token_logprobs ({K} alternatives)", 1, lambda: token_logprobs(x, y, top_k=K)),
+            ("token_logprobs_bwd", 2, lambda: token_logprobs_bwd(x, y, scored, stats, g, g, None, 1.0, grad)),
+            (f"distill_topk_fwd_bwd ({K} entries)", 2,
+             lambda: distill_topk_fwd_bwd_(x, out.top_logprobs, out.top_ids, 1.0, tail="bucket", out=grad))):
+        ms = time_cuda(fn, iters=10)
+        _ext.check_status()
+        gbs = passes * x.numel() * 2 / ms / 1e6
+        recs.append({"kernel": name, "shape": [rows, V], "ms": round(ms, 4), "gbs": round(gbs, 1),
+                     "frac_of_copy_rate": round(gbs / peaks()["gbs"], 3)})
+    return recs
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser()
     ap.add_argument("--quick", action="store_true")
@@ -169,6 +194,7 @@ def main(argv=None):
     ap.add_argument("--attn-warmup", type=int, default=3)
     ap.add_argument("--zero", action="store_true", help="also time the optimizer step kernel")
     ap.add_argument("--fused", action="store_true", help="also time the bandwidth-bound kernels of a Llama block")
+    ap.add_argument("--head", action="store_true", help="also time the operators on rows of logits")
     args = ap.parse_args(argv)
     shapes = [(8192, 8192, 8192, False, False)]
     if not args.quick:
@@ -185,6 +211,9 @@ def main(argv=None):
         print(json.dumps(bench_zero()), flush=True)
     if args.fused:
         for rec in bench_fused():
+            print(json.dumps(rec), flush=True)
+    if args.head:
+        for rec in bench_head():
             print(json.dumps(rec), flush=True)
     if not args.no_attn:
         for S in (args.seq or ([8192] if args.quick else [8192, 32768])):

@@ -523,6 +523,22 @@ void check_logits(const Tensor& t) {
   TORCH_CHECK(t.size(0) <= INT32_MAX && t.size(1) <= zx::kHeadMaxVocab, "logits: at most 2^31 - 1 rows and ",
               zx::kHeadMaxVocab, " columns");
 }
+// First byte and the one behind the last of [rows, ...] with contiguous columns.
+std::pair<const char*, const char*> bytes_of(const Tensor& t) {
+  const char* p = static_cast<const char*>(t.data_ptr());
+  if (t.numel() == 0) return {p, p};
+  if (t.is_contiguous()) return {p, p + t.nbytes()};
+  const int64_t step = t.size(0) > 1 ? t.stride(0) : 0;
+  return {p, p + ((t.size(0) - 1) * step + t.size(1)) * t.element_size()};
+}
+bool apart(const Tensor& a, const Tensor& b) {
+  const auto x = bytes_of(a), y = bytes_of(b);
+  return x.second <= y.first || y.second <= x.first;
+}
+// What else a kernel reads while it writes the gradient.
+void check_apart(const Tensor& d, const c10::optional<Tensor>& t, const char* name) {
+  TORCH_CHECK(!t.has_value() || apart(d, *t), "d_logits overlaps ", name);
+}
 // A gradient that is written: rows must not share memory, and it may be the logits but not overlap them otherwise.
 void check_dlogits(const Tensor& d, const Tensor& x) {
   TORCH_CHECK(d.sizes() == x.sizes() && d.scalar_type() == x.scalar_type() && d.device() == x.device(),
@@ -530,14 +546,8 @@ void check_dlogits(const Tensor& d, const Tensor& x) {
   TORCH_CHECK(d.size(1) == 1 || d.stride(1) == 1, "d_logits must have contiguous columns");
   TORCH_CHECK(d.size(0) <= 1 || d.stride(0) >= d.size(1), "the rows of d_logits share memory");
   if (d.numel() == 0) return;
-  auto ends = [](const Tensor& t) {
-    const char* p = static_cast<const char*>(t.data_ptr());
-    const int64_t step = t.size(0) > 1 ? t.stride(0) : 0;
-    return std::pair<const char*, const char*>(p, p + ((t.size(0) - 1) * step + t.size(1)) * t.element_size());
-  };
-  const auto a = ends(d), b = ends(x);
-  const bool same = a.first == b.first && (d.size(0) == 1 || d.stride(0) == x.stride(0));
-  TORCH_CHECK(same || a.second <= b.first || b.second <= a.first,
+  const bool same = d.data_ptr() == x.data_ptr() && (d.size(0) == 1 || d.stride(0) == x.stride(0));
+  TORCH_CHECK(same || apart(d, x),
               "d_logits overlaps the logits without being the same tensor");
 }
 const float* float_rows(const c10::optional<Tensor>& t, int64_t n, const Tensor& like, const char* name) {
@@ -617,6 +627,13 @@ void token_logprobs_bwd(const Tensor& logits, const c10::optional<Tensor>& targe
     a.top_ids = (int64_t*)id_array(*top_ids, (int64_t)a.rows * a.top_k, logits, "top_ids").p;
     a.d_top = float_rows(d_top, (int64_t)a.rows * a.top_k, logits, "d_top");
   }
+  check_apart(d_logits, targets, "the targets");
+  check_apart(d_logits, top_ids, "top_ids");
+  check_apart(d_logits, d_top, "d_top");
+  check_apart(d_logits, d_logprobs, "d_logprobs");
+  check_apart(d_logits, d_entropy, "d_entropy");
+  check_apart(d_logits, entropy, "the entropy");
+  check_apart(d_logits, stats, "stats");
   a.d_logits = d_logits.data_ptr();
   a.d_ld = d_logits.stride(0);
   c10::cuda::CUDAGuard guard(logits.device());
@@ -656,6 +673,11 @@ void distill_topk(const Tensor& logits, const Tensor& values, const Tensor& ids,
   a.d_loss = float_rows(d_loss, a.rows, logits, "d_loss");
   if (d_logits.has_value()) {
     check_dlogits(*d_logits, logits);
+    check_apart(*d_logits, values, "the teacher's values");
+    check_apart(*d_logits, ids, "the teacher's ids");
+    check_apart(*d_logits, loss, "the losses");
+    check_apart(*d_logits, stats, "stats");
+    check_apart(*d_logits, d_loss, "d_loss");
     a.d_logits = d_logits->data_ptr();
     a.d_ld = d_logits->stride(0);
   }

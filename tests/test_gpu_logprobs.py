@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import _logprobs_oracle as oracle
-from zenyx_b200.ops import _ext
+from zenyx_b200.ops import _ext, logprobs as ops
 from zenyx_b200.ops.logprobs import MAX_VOCAB, distill_topk, distill_topk_fwd_bwd_, token_logprobs
 
 pytestmark = pytest.mark.gpu
@@ -596,3 +596,19 @@ def test_scoring_without_gradients_is_scoring_with_them():
         distill_topk_fwd_bwd_(z, without.top_logprobs, without.top_ids, 1.0)
     for a, b in zip(with_grad, without):
         assert torch.equal(a, b)
+
+
+def test_gradients_that_lie_across_other_arguments_are_refused():
+    buffer = torch.zeros(4, 120, device="cuda")
+    x, y = torch.randn(4, 100, device="cuda"), torch.zeros(4, device="cuda", dtype=torch.int64)
+    ids = torch.arange(8, device="cuda").view(4, 2)
+    flat = buffer.view(-1)
+    with pytest.raises(RuntimeError, match="values"):
+        distill_topk_fwd_bwd_(x, flat[200:208].view(4, 2), ids, 1.0, out=buffer[:, :100])
+    with pytest.raises(RuntimeError, match="ids"):
+        distill_topk_fwd_bwd_(x, torch.zeros(4, 2, device="cuda"), flat[:8].view(torch.int32).view(4, 2), 1.0, out=buffer[:, :100])
+    out, stats = ops.token_logprobs_fwd(x, y, 2, 1.0)
+    with pytest.raises(RuntimeError, match="d_entropy"):
+        ops.token_logprobs_bwd(x, y, out, stats, None, flat[101:105], None, 1.0, buffer[:, 20:])
+    # beside one another is fine
+    distill_topk_fwd_bwd_(x, flat[470:478].view(4, 2), ids, 1.0, out=buffer.view(-1)[:400].view(4, 100))

@@ -130,7 +130,7 @@ class Trainer:
                      temperature: float = 1.0, tail: str = "renormalize") -> float:
         """One optimizer step of the flagship on what a teacher wrote down for the same tokens: ``teacher_logprobs`` and
         ``teacher_ids`` [global_batch, seq_len, K] from ``LlamaModel.token_logprobs(top_k=K)``. Returns the global mean
-        divergence. What the loss is: ``ops.logprobs.distill_topk``."""
+        divergence (positions that the teacher left out count as 0). What the loss is: ``ops.logprobs.distill_topk``."""
         if self.engine is None:
             raise ValueError("distill_step needs the flagship path: Trainer(LlamaConfig, ...)")
         return self._engine_step(lambda: self.engine.distill_step(tokens, teacher_logprobs, teacher_ids, lr=self._lr(),

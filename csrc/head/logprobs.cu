@@ -143,11 +143,27 @@ __device__ __forceinline__ int above_in_run(const uint64_t* run, uint64_t key) {
     if (run[c + step - 1] > key) c += step;
   return c + (run[c] > key ? 1 : 0);
 }
-// best[0 .. k) = the k largest of list[0 .. n), in order (0 where there are fewer): runs of 32 are sorted, each by a warp;
-// a member's place is its own in the run plus, in each other run, the number above it. Needs a barrier before.
+// best[0 .. k) = the k largest of list[0 .. n), in order (0 where there are fewer). Needs a barrier before, ends with one.
+// Up to 128 members: each counts those above it, with the help of neighbouring lanes. More: runs of 32 are sorted, each by
+// a warp; a member's place is its own in the run plus, in each other run, the number above it.
 __device__ __forceinline__ void rank_list(TopShared& sh, int n, int k) {
   const int tid = threadIdx.x, nt = blockDim.x, runs = (n + 31) / 32;
-  for (int i = tid; i < k; i += nt) sh.best[i] = 0;
+  for (int i = n + tid; i < k; i += nt) sh.best[i] = 0;
+  if (n <= 128) {
+    const int shift = min(5, max(0, 31 - __clz(nt / max(n, 1)))), lanes = 1 << shift;      // for one member
+    const int part = tid & (lanes - 1);
+    for (int first = 0; first < n; first += nt >> shift) {
+      const int at = first + (tid >> shift);
+      const uint64_t mine = at < n ? sh.list[at] : ~0ull;
+      int r = 0;
+#pragma unroll 4
+      for (int i = part; i < n; i += lanes) r += sh.list[i] > mine;
+      for (int o = lanes / 2; o > 0; o /= 2) r += __shfl_xor_sync(0xffffffffu, r, o);
+      if (part == 0 && at < n && r < k) sh.best[r] = mine;
+    }
+    __syncthreads();
+    return;
+  }
   for (int i = tid; i < runs * 32; i += nt) sh.list[i] = warp_sort(i < n ? sh.list[i] : (uint64_t)0);
   if (tid < 32) sh.list[runs * 32 + tid] = 0;      // an empty run behind the last
   __syncthreads();
@@ -165,21 +181,34 @@ __device__ __forceinline__ void rank_list(TopShared& sh, int n, int k) {
   __syncthreads();
 }
 
+// Where a thread's `mine` entries start in a list of *n so far: one atomic a warp.
+__device__ __forceinline__ int take_places(int* n, int mine) {
+  const int lane = threadIdx.x & 31;
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += up;
+  }
+  int first = 0;
+  if (lane == 31 && upto > 0) first = atomicAdd(n, upto);
+  return __shfl_sync(0xffffffffu, first, 31) + upto - mine;
+}
+
 // The same of `lists` sorted lists of k each (of the blocks of a cluster).
 __device__ __forceinline__ void merge_lists(TopShared& sh, const uint64_t* list, int lists, int k) {
   // The k-th is not below the smallest of the lists' members number ceil(k / lists), nor below any list's last.
-  const int q = (k + lists - 1) / lists;
-  uint64_t least = ~0ull, lo = 1;
-  for (int b = 0; b < lists; ++b) {
-    least = min(least, list[b * k + q - 1]);
-    lo = max(lo, list[b * k + k - 1]);
-  }
-  lo = max(lo, least);
+  const int q = (k + lists - 1) / lists, lane = threadIdx.x & 31;
+  const bool one = lane < lists;
+  const uint32_t least = __reduce_min_sync(0xffffffffu, one ? (uint32_t)(list[lane * k + q - 1] >> 32) : 0xffffffffu);
+  const uint32_t last = __reduce_max_sync(0xffffffffu, one ? (uint32_t)(list[lane * k + k - 1] >> 32) : 0);
+  const uint64_t lo = max((uint64_t)max(least, last) << 32, (uint64_t)1);
   if (threadIdx.x == 0) sh.n = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < lists * k; i += blockDim.x) {
-    const uint64_t key = list[i];
-    if (key >= lo) sh.list[atomicAdd(&sh.n, 1)] = key;
+  for (int i = threadIdx.x; i - (int)(threadIdx.x & 31) < lists * k; i += blockDim.x) {   // whole warps
+    const uint64_t key = i < lists * k ? list[i] : 0;
+    const int at = take_places(&sh.n, key >= lo);
+    if (key >= lo) sh.list[at] = key;
   }
   __syncthreads();
   rank_list(sh, sh.n, k);
@@ -273,6 +302,7 @@ struct FwdShared {
   float m;
   double log_l;
   uint32_t least[4][kWarps], most[kWarps];
+  __align__(16) uint32_t own[kThreads];
 };
 
 // One group of vectors into the running sums (l and s as pairs).
@@ -420,11 +450,19 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(LogprobsArgs 
   t = warp_join(t, c2);
   if (lane == 0) sh.part[warp] = t;
   if (TOP) {
-    const uint32_t sorted = warp_sort(own);
+    // What ceil(K / 2^j) of the warp's threads reach: the smallest that fewer are above.
+    sh.own[tid] = own;
+    __syncwarp();
+    int above = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {       // what ceil(K / 2^j) of the warp's threads reach
+    for (int i = 0; i < 8; ++i) {
+      const uint4 o = reinterpret_cast<const uint4*>(&sh.own[warp * 32])[i];
+      above += (o.x > own) + (o.y > own) + (o.z > own) + (o.w > own);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
       const int q = (K + (1 << j) - 1) >> j;
-      const uint32_t least = __shfl_sync(0xffffffffu, sorted, min(q, 32) - 1);
+      const uint32_t least = __reduce_min_sync(0xffffffffu, above < q ? own : 0xffffffffu);
       if (lane == 0) sh.least[j][warp] = q <= 32 ? least : 0;
     }
     if (lane == 0) {
@@ -504,27 +542,28 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(LogprobsArgs 
         join();
         joined = true;
       }
-      for (int i = tid; i < total && tid < hands; i += 2 * hands) {
+      for (int first = warp * 32; first < total && tid < hands; first += 2 * hands) {
         uint4 v[2];
         int vec[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const int at = i + u * hands, g = top.group[min(at, total - 1) / kUnroll];
+          const int at = first + lane + u * hands, g = top.group[min(at, total - 1) / kUnroll];
           vec[u] = v0 + ((g >> 16) * kUnroll + at % kUnroll) * nt + (g & 0xffff);
           v[u] = at < total ? row.load(vec[u], v1) : Vec<T>::nothing();
         }
+        constexpr int N = Vec<T>::N;
+        uint32_t hits = 0;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          if (!(Vec<T>::max_of(Vec<T>::max_w(v[u])) >= bound)) continue;
-          const T* e = reinterpret_cast<const T*>(&v[u]);
-#pragma unroll
-          for (int j = 0; j < Vec<T>::N; ++j) {
-            const float x = to_f(e[j]);
-            if (x >= bound) {
-              const int at = atomicAdd(&top.n, 1);
-              if (at < kCandidates) top.list[at] = alt_key(order_key(x), row.col(vec[u]) + j);
-            }
-          }
+        for (int i = 0; i < 2 * N; ++i)
+          hits |= to_f(reinterpret_cast<const T*>(&v[i / N])[i % N]) >= bound ? 1u << i : 0u;
+        int at = take_places(&top.n, __popc(hits));
+        for (; __any_sync(0xffffffffu, hits != 0); hits &= hits - 1) {
+          if (hits == 0) continue;
+          const int i = __ffs(hits) - 1;
+          const uint4 w = i < N ? v[0] : v[1];
+          const float x = Vec<T>::one(w, i % N);
+          if (at < kCandidates) top.list[at] = alt_key(order_key(x), row.col(i < N ? vec[0] : vec[1]) + i % N);
+          ++at;
         }
       }
       __syncthreads();

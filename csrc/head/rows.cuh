@@ -141,6 +141,18 @@ struct Vec {
       w[2 * i + 1] = __float_as_uint(b);
     }
   }
+  // Element i of a vector in registers.
+  static __device__ __forceinline__ float one(const uint4& v, int i) {
+    const int word = Elem<T>::kPerWord == 2 ? i >> 1 : i;
+    const uint32_t a = word & 1 ? v.y : v.x, b = word & 1 ? v.w : v.z, w = word & 2 ? b : a;
+    if constexpr (Elem<T>::kPerWord == 2) {
+      float lo, hi;
+      unpair(Elem<T>::wide(w), lo, hi);
+      return i & 1 ? hi : lo;
+    } else {
+      return __uint_as_float(w);
+    }
+  }
   static __device__ __forceinline__ uint32_t max_w(const uint4& v) {
     return Elem<T>::max_w(Elem<T>::max_w(v.x, v.y), Elem<T>::max_w(v.z, v.w));
   }

@@ -135,6 +135,8 @@ __device__ __forceinline__ uint32_t find_bound(TopShared& sh, const uint32_t* gr
   return lo;
 }
 
+__device__ __forceinline__ void first_threads_sync(int n) { asm volatile("bar.sync 1, %0;" ::"r"(n) : "memory"); }
+
 // How many of the 32 keys at run (descending) are above key.
 __device__ __forceinline__ int above_in_run(const uint64_t* run, uint64_t key) {
   int c = 0;
@@ -146,8 +148,9 @@ __device__ __forceinline__ int above_in_run(const uint64_t* run, uint64_t key) {
 // best[0 .. k) = the k largest of list[0 .. n), in order (0 where there are fewer). Needs a barrier before, ends with one.
 // Up to 128 members: each counts those above it, with the help of neighbouring lanes. More: runs of 32 are sorted, each by
 // a warp; a member's place is its own in the run plus, in each other run, the number above it.
-__device__ __forceinline__ void rank_list(TopShared& sh, int n, int k) {
-  const int tid = threadIdx.x, nt = blockDim.x, runs = (n + 31) / 32;
+// Called by the first nt threads.
+__device__ __forceinline__ void rank_list(TopShared& sh, int n, int k, int nt) {
+  const int tid = threadIdx.x, runs = (n + 31) / 32;
   for (int i = n + tid; i < k; i += nt) sh.best[i] = 0;
   if (n <= 128) {
     const int shift = min(5, max(0, 31 - __clz(nt / max(n, 1)))), lanes = 1 << shift;      // for one member
@@ -161,12 +164,12 @@ __device__ __forceinline__ void rank_list(TopShared& sh, int n, int k) {
       for (int o = lanes / 2; o > 0; o /= 2) r += __shfl_xor_sync(0xffffffffu, r, o);
       if (part == 0 && at < n && r < k) sh.best[r] = mine;
     }
-    __syncthreads();
+    first_threads_sync(nt);
     return;
   }
   for (int i = tid; i < runs * 32; i += nt) sh.list[i] = warp_sort(i < n ? sh.list[i] : (uint64_t)0);
   if (tid < 32) sh.list[runs * 32 + tid] = 0;      // an empty run behind the last
-  __syncthreads();
+  first_threads_sync(nt);
   for (int i = tid; i < runs * 32; i += nt) {
     const uint64_t mine = sh.list[i];
     int r = i & 31;
@@ -178,7 +181,7 @@ __device__ __forceinline__ void rank_list(TopShared& sh, int n, int k) {
     }
     if (r < k) sh.best[r] = mine;
   }
-  __syncthreads();
+  first_threads_sync(nt);
 }
 
 // Where a thread's `mine` entries start in a list of *n so far: one atomic a warp.
@@ -195,8 +198,8 @@ __device__ __forceinline__ int take_places(int* n, int mine) {
   return __shfl_sync(0xffffffffu, first, 31) + upto - mine;
 }
 
-// The same of `lists` sorted lists of k each (of the blocks of a cluster).
-__device__ __forceinline__ void merge_lists(TopShared& sh, const uint64_t* list, int lists, int k) {
+// The same of `lists` sorted lists of k each (of the blocks of a cluster). Called by the first nt threads.
+__device__ __forceinline__ void merge_lists(TopShared& sh, const uint64_t* list, int lists, int k, int nt) {
   // The k-th is not below the smallest of the lists' members number ceil(k / lists), nor below any list's last.
   const int q = (k + lists - 1) / lists, lane = threadIdx.x & 31;
   const bool one = lane < lists;
@@ -204,14 +207,14 @@ __device__ __forceinline__ void merge_lists(TopShared& sh, const uint64_t* list,
   const uint32_t last = __reduce_max_sync(0xffffffffu, one ? (uint32_t)(list[lane * k + k - 1] >> 32) : 0);
   const uint64_t lo = max((uint64_t)max(least, last) << 32, (uint64_t)1);
   if (threadIdx.x == 0) sh.n = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i - (int)(threadIdx.x & 31) < lists * k; i += blockDim.x) {   // whole warps
+  first_threads_sync(nt);
+  for (int i = threadIdx.x; i - (int)(threadIdx.x & 31) < lists * k; i += nt) {   // whole warps
     const uint64_t key = i < lists * k ? list[i] : 0;
     const int at = take_places(&sh.n, key >= lo);
     if (key >= lo) sh.list[at] = key;
   }
-  __syncthreads();
-  rank_list(sh, sh.n, k);
+  first_threads_sync(nt);
+  rank_list(sh, sh.n, k, nt);
 }
 
 // Any input, ties without end: the k-th largest value by its digits (four passes of 8 bits), then everything above it and
@@ -575,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(LogprobsArgs 
       }
     }
     if (warp == warps - 1 && !joined) join();
-    rank_list(top, n, K);
+    rank_list(top, n, K, nt);
     if (cluster > 1)
       for (int k = tid; k < K; k += nt) store_to_cta(&lists[rank * K + k], 0, top.best[k]);
   }
@@ -583,14 +586,17 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(LogprobsArgs 
     cluster_arrive();
     cluster_wait();
     if (rank != 0) return;
+    // the last warp has the row's sums to see to, the others the lists
+    const int hands = TOP && warps > 1 ? nt - 32 : nt;
+    if (TOP && tid < hands) merge_lists(top, lists, cluster, K, hands);
     if (warp == warps - 1) {
       Sums b = lane < cluster ? Sums{sh.cta[lane][0], sh.cta[lane][1], sh.cta[lane][2]} : Sums{-FLT_MAX, 0.f, 0.f};
       tell(warp_join(b, c2));
     }
-    if (TOP) merge_lists(top, lists, cluster, K);
+    if (TOP) __syncthreads();
   }
   if (!TOP) return;
-  // (rank_list and merge_lists end with a barrier: what tell() left is there)
+  // (there was a barrier since tell())
   const bool bad = is_bad(sh.m);
   for (int k = tid; k < K; k += nt) {
     const uint64_t key = bad ? 0 : top.best[k];

@@ -612,3 +612,27 @@ def test_gradients_that_lie_across_other_arguments_are_refused():
         ops.token_logprobs_bwd(x, y, out, stats, None, flat[101:105], None, 1.0, buffer[:, 20:])
     # beside one another is fine
     distill_topk_fwd_bwd_(x, flat[470:478].view(4, 2), ids, 1.0, out=buffer.view(-1)[:400].view(4, 100))
+
+
+def test_small_results_are_tensors_of_their_own():
+    x, y, _ = _logits(3, 50, torch.bfloat16)
+    first = token_logprobs(x, y, top_k=2)
+    kept = [t.clone() for t in first]
+    second = token_logprobs(x.flip(1), y, top_k=2)
+    assert all(torch.equal(a, b) for a, b in zip(first, kept))
+    second.logprobs.fill_(5.0)
+    second.top_ids.zero_()
+    assert bool((second.entropy != 5.0).all()) and bool((second.top_logprobs != 0.0).any())
+    for t in (*first, *second):
+        assert t.is_contiguous() and t.data_ptr() % 16 == 0 and t._base is None
+    a = x.clone().requires_grad_(True)
+    out = token_logprobs(a, y, top_k=2)
+    with torch.no_grad():
+        out.top_ids[0, 0] += 0                      # what the backward has kept: noticed
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.logprobs.sum().backward()
+    out = token_logprobs(a, y, top_k=2)
+    out.logprobs.detach().zero_()                   # what it has not: nothing to it
+    (out.entropy.sum() + out.logprobs.sum()).backward()
+    want, off = oracle.logprobs_grad(x, y, 0, 1.0, torch.ones(3, device="cuda"), torch.ones(3, device="cuda"), None)
+    oracle.check(a.grad, want, off, "gradient")

@@ -93,7 +93,8 @@ __device__ __forceinline__ Teacher weigh(const DistillArgs& a, Entries& e) {
 }
 // The entries' weights with those of the same token added up, and whether an entry is the first with its token.
 // Entries are few: each looks at all. s_id, s_w: [kHeadMaxTop] in shared memory for this warp.
-__device__ __noinline__ void join_same(const Entries& e, int K, int* s_id, float* s_w, float (&q_all)[kEntries], bool (&first)[kEntries]) {
+__device__ __noinline__ void join_same(const Entries& e, int K, int* s_id, float* s_w, float (&q_all)[kEntries],
+                                       bool (&first)[kEntries]) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int i = 0; i < kEntries; ++i) {
@@ -522,7 +523,8 @@ __global__ void __launch_bounds__(kWorkers + 32, 6) distill_kernel(DistillArgs a
       }
       const int xc = live_rows & 1;
       if (cluster > 1) {
-        if (lane < cluster) send(map_to_cta(&sh.outside[xc][rank * kWorkerWarps + warp], lane), map_to_cta(&sh.exchanged[xc], lane), mr, lr);
+        if (lane < cluster)
+          send(map_to_cta(&sh.outside[xc][rank * kWorkerWarps + warp], lane), map_to_cta(&sh.exchanged[xc], lane), mr, lr);
         __syncwarp();
       } else {
         if (lane == 0) sh.outside[xc][warp] = make_float2(mr, lr);
@@ -639,7 +641,8 @@ __global__ void __launch_bounds__(kWorkers + 32, 6) distill_kernel(DistillArgs a
 // ------------------------------------------------------------------------------------------
 // Gradient from the forward's statistics, one block a segment of a row. The first warps hold the teacher's entries.
 // ------------------------------------------------------------------------------------------
-constexpr int kThreads = 256;   // (128: 365 us instead of 317 for 4096 x 128256 bf16: the entries are a warp's work in each block)
+// Blocks of 128 threads: 365 us instead of 317 for 4096 x 128256 bf16 (the entries are a warp's work in each block).
+constexpr int kThreads = 256;
 constexpr int kGradVecs = 8;    // vectors of a thread, all in flight
 
 template <class T>
@@ -726,10 +729,11 @@ __global__ void __launch_bounds__(kThreads, 4) distill_bwd_kernel(DistillArgs a,
 // Launches
 // ------------------------------------------------------------------------------------------
 // Blocks a row. What counts is how many bytes of slices an SM holds, and then how few blocks they are in (each has its
-// fixed work): the largest sum over four to six blocks, fewer blocks unless more hold a sixteenth more. 4096 x 128256 bf16: six blocks a row (five slices of 43 KB on an
-// SM) 392 us, five 403, four and eight (192 KB held) 437 and 433; 4000 x 50257: two (four of 50 KB) 163, three (six of
-// 34 KB) 181, one (two of 100 KB) 192, four (six of 25 KB) 196; 4096 x 32000 fp32: three 170, two and four 173.
-// Five and seven are left out: seven measured 262 us where six took 243 (2048 x 151936), five never was the best.
+// fixed work): the largest sum over four to six blocks, fewer blocks unless more hold a sixteenth more.
+// 4096 x 128256 bf16: six blocks a row (five slices of 43 KB on an SM) 392 us, five 403, four and eight (192 KB held) 437
+// and 433; 4000 x 50257: two (four of 50 KB) 163, three (six of 34 KB) 181, one (two of 100 KB) 192, four (six of 25 KB) 196;
+// 4096 x 32000 fp32: three 170, two and four 173. Five and seven are left out: seven measured 262 us where six took 243
+// (2048 x 151936), five never was the best.
 // Few rows are split further, as long as the grid stays below five blocks an SM and a worker has a vector: 150 x 50257 takes
 // 15.3 us with four blocks a row, 16.3 with two, 19.1 with eight.
 int blocks_a_row(int vecs, int rows, int sm_count) {

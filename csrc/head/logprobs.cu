@@ -5,10 +5,10 @@
 // z_j - lse = ln 2 (d_j - log2 l), H = ln 2 (log2 l - s / l), in which both terms are >= 0, so nothing cancels. (maximum, l)
 // is what the backward needs. Sums are held in 32 bits, the few scalars of a row are put together in 64.
 //
-// Measured on a B200 that copies 6557 GB/s: forward 4096 x 128256 bf16 161 us (6.5 TB/s), with 20 alternatives 203, 64
-// 219, 128 254; one row 4.5 us, with 20 alternatives 9.0 (launch and the search's chain of barriers); 64 x 128256 fp32
-// 10.2 us (3.2 TB/s: a cluster's start and end are as long as its slice). Backward 2048 x 128256 bf16 159 us (6.6 TB/s),
-// 4096 rows with 64 alternatives 334.
+// Measured on a B200 that copies 6557 GB/s: forward 4096 x 128256 bf16 161 us (6.5 TB/s), with 20 alternatives 200, 64
+// 218, 128 243; one row 4.5 us, with 20 alternatives 7.6 (launch and the search's chain of barriers); 64 x 128256 fp32
+// 10.2 us (3.2 TB/s: a cluster's start and end are as long as its slice), with 20 alternatives 15.3. Backward 2048 x 128256
+// bf16 159 us (6.6 TB/s), 4096 rows with 64 alternatives 334.
 #include <algorithm>
 #include "rows.cuh"
 
@@ -146,7 +146,8 @@ __device__ __forceinline__ int above_in_run(const uint64_t* run, uint64_t key) {
   return c + (run[c] > key ? 1 : 0);
 }
 // best[0 .. k) = the k largest of list[0 .. n), in order (0 where there are fewer). Needs a barrier before, ends with one.
-// Up to 128 members: each counts those above it, with the help of neighbouring lanes. More: runs of 32 are sorted, each by
+// Up to 128 members: each counts those above it, with the help of neighbouring lanes (one row, 20 alternatives: 8.0 us with
+// this, 9.0 with runs alone; for more members the runs take fewer steps). More: runs of 32 are sorted, each by
 // a warp; a member's place is its own in the run plus, in each other run, the number above it.
 // Called by the first nt threads.
 __device__ __forceinline__ void rank_list(TopShared& sh, int n, int k, int nt) {
@@ -349,8 +350,9 @@ __device__ __forceinline__ void add_group(const uint4 (&v)[U], float M, float c2
 // more than 2 k + 32 groups pass, a histogram of the group maxima gives a better one (always: 4096 x 128256, one
 // alternative, 206 us instead of 191; never: 999 x 50257 fp16, 128 alternatives, 79 instead of 45); where that does not
 // help either (ties, large logits side by side), the k are selected by their digits from all of the row.
-// What the search costs is its chain of barriers and reads, in which a block asks for little: 8 us of a row's 29 at 4096 x
-// 128256. Copies into shared memory ahead of their use (a ring for each warp) made it 242 us instead of 219, larger steps
+// What the search costs is its chain of barriers and reads, in which a block asks for little: 7 us of a row's 29 at 4096 x
+// 128256. Of the 13,800 clocks that one row with 20 alternatives takes, 3500 are the scan, 1300 sums and bound, 550 the list
+// of groups, 2000 the second look, 1200 the order, 1200 the exchange in the cluster, 2500 the merge. Copies into shared memory ahead of their use (a ring for each warp) made it 242 us instead of 219, larger steps
 // 240, the next row's start in the L2 cache 227.
 template <class T, bool TOP>
 __global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(LogprobsArgs a, int cluster, int steps) {

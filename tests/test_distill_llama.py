@@ -116,3 +116,44 @@ def test_trainer_distill_step_on_the_gpu():
         assert loss == loss and loss > 0
     _ext.check_status()
     trainer.close()
+
+
+def _distill_ranks(rank, world, cp, tmp):
+    """Replicas, or one sequence over a ring: the tokens and what the teacher wrote down are cut the same way, so the loss
+    and the scores are a single process's."""
+    from zenyx_b200.ops.attention import shard_sequence
+
+    cfg = LlamaConfig.tiny(n_layers=1, d_model=64, n_heads=2, n_kv_heads=1, ffn_dim=96, vocab_size=128)
+    S = 512
+    tokens = _tokens(2, S)
+    teacher = LlamaModel(cfg, device="cpu", dtype=torch.float32, seed=9)
+    wrote = teacher.token_logprobs(tokens, top_k=4)
+    ids = wrote.top_ids.clone()
+    ids[0, 30:50] = -1
+    trainer = Trainer(cfg, TrainerConfig(lr=1e-2, seq_len=S, global_batch=2, ring_degree=cp, max_grad_norm=1.0, seed=4))
+    ring = trainer.engine.ring
+    if cp > 1:
+        part = shard_sequence(tokens, ring.rank, cp, ring.layout)
+        scores = trainer.model.token_logprobs(part, part, top_k=2, ring=ring)
+        torch.save(tuple(scores), f"{tmp}/scores{rank}.pt")
+    losses = [trainer.distill_step(tokens, wrote.top_logprobs, ids, tail="bucket") for _ in range(2)]
+    torch.save((losses, trainer.model.w("lm_head.weight").clone(), ring.rank, ring.layout), f"{tmp}/{cp}_{world}_{rank}.pt")
+    trainer.close()
+
+
+@pytest.mark.parametrize("cp", [1, 2])
+def test_distillation_on_two_ranks_is_that_of_one(tmp_path, cp):
+    import test_dist_cpu
+
+    test_dist_cpu.run_ranks(_distill_ranks, world=2, args=(cp, str(tmp_path)))
+    _distill_ranks(0, 1, 1, str(tmp_path))
+    one = torch.load(tmp_path / "1_1_0.pt")
+    for rank in range(2):
+        losses, head, *_ = torch.load(tmp_path / f"{cp}_2_{rank}.pt")
+        # bf16 weights and activations in another order of sums: 2^-8 of a loss of a few units, twice that after a step
+        assert max(abs(a - b) for a, b in zip(losses, one[0])) < 2 * 2.0 ** -8 * max(one[0])
+        assert (head.float() - one[1].float()).abs().max() <= 3 * 1e-2      # two steps of Adam move a weight by lr each
+    if cp == 2:
+        for rank in range(2):
+            scores = torch.load(tmp_path / f"scores{rank}.pt")
+            assert scores[0].shape == (2, 256) and scores[3].shape == (2, 256, 2) and bool(torch.isfinite(scores[0]).all())

@@ -259,7 +259,7 @@ __device__ __noinline__ void select_exactly(TopShared& sh, const Row<T>& row, in
   }
   if (prefix <= kNegInfKey) prefix = kNegInfKey;   // fewer than k: all that there are are above it
   if (tid == 0) sh.n = 0;
-  int ties = 0;   // of those before this round's vectors
+  int ties = 0;   // of those before the vectors at hand
   __syncthreads();
   for (int base = v0; base < v1; base += blockDim.x) {
     const int i = base + tid;

@@ -2,7 +2,9 @@
 // p = softmax(z), teacher values v_k at the columns i_k:
 //   renormalize: q = softmax(v);                    loss = sum q_k (log q_k - log p_{i_k})
 //   bucket:      q = exp(v), q_r = max(0, 1 - sum q), p_r = the sum of p outside the columns;   + q_r (log q_r - log p_r)
-//   temperature dloss/dx_j = p_j - q_j  (bucket, outside the columns: p_j (1 - q_r / p_r))
+//   temperature dloss/dx_j = s p_j - q_j  (bucket, outside the columns: p_j (s - q_r / p_r))
+// where s is the sum of the weights in the loss: 1, but sum q where a bucket has nothing left (rounded values may add up to
+// more than 1) or where the student has nothing outside, so that the bucket's part is not in the loss.
 // Bound by the bytes of the logits, read once, and of the gradient. Measured on a B200 that copies 6557 GB/s, 64 of the
 // teacher's tokens: loss and gradient of 4096 x 128256 bf16 391 us (5.4 TB/s), 4096 x 32000 fp32 168 (6.2), 4000 x 50257
 // bf16 161 (5.0), 256 x 512 7.0 us; the loss alone of 4096 x 128256 227 us (4.6), its gradient from the statistics 317 (6.6).
@@ -131,14 +133,14 @@ __device__ __noinline__ void join_same(const Entries& e, int K, int* s_id, float
 //
 // The teacher's columns are kept apart so that the sum over all others is taken relative to their own maximum: the mass
 // outside keeps its digits when the teacher's tokens have nearly all of it.
-// stats = (maximum outside, coefficient of 2^d outside, maximum, 1 / l); the last is -1 for a row that is left out.
+// stats = (maximum outside, coefficient of 2^d outside, maximum, s / l); the last is -1 for a row that is left out.
 constexpr int kWorkers = 128;
 constexpr int kWorkerWarps = kWorkers / 32;
 constexpr int kCopy = 8192;    // bytes of one asynchronous copy
 
 struct alignas(16) TeacherPart {   // of the teacher's tokens in a block's slice; moved in stores of 16 bytes
-  float mt, lt, none[2];           // maximum, sum relative to it
-  double terms, weight;            // sum of q_k (log q_k - ln 2 rel2(x_k)), sum of q_k
+  float mt, lt, q, none;           // maximum, sum relative to it, sum of q_k
+  double terms, weight;            // in the first block: sum of q_k (log q_k - ln 2 rel2(x_k)), sum of q_k
 };
 struct DistillShared {
   uint64_t full, ready, empty, exchanged[2], answered, told[2], taken[2];
@@ -375,13 +377,13 @@ __device__ __forceinline__ void distill_auxiliary(const DistillArgs& a, DistillS
       if (cluster > 1) {
         if (lane < cluster) {
           const uint32_t to = map_to_cta(&sh.teacher[xc][rank], lane), bar = map_to_cta(&sh.exchanged[xc], lane);
-          send(to, bar, mt, lt, 0.f, 0.f);
+          send(to, bar, mt, lt, (float)weight, 0.f);
           if (lane == 0) send(to + 16, bar, terms, weight);
         }
         __syncwarp();
       } else {
         // launched without a cluster: such a store is not allowed there, not even to the block itself
-        if (lane == 0) sh.teacher[xc][0] = TeacherPart{mt, lt, {0.f, 0.f}, terms, weight};
+        if (lane == 0) sh.teacher[xc][0] = TeacherPart{mt, lt, (float)weight, 0.f, terms, weight};
         mbar_arrive_warp(&sh.exchanged[xc]);
       }
     } else {
@@ -563,7 +565,12 @@ __global__ void __launch_bounds__(kWorkers + 32, 6) distill_kernel(DistillArgs a
       else join(gap2_far(part.x, mr, c2), gap2_far(tm, m, c2), gap2_far(mr, m, c2));
       const float l = lt + lr * share;
       const bool bad = is_bad(m);
-      const float inv_l = bad ? nan_f() : (l == 0.f ? 0.f : 1.f / l);
+      float weights = 1.f;      // s
+      if (a.bucket && !(q_rest > 0.f && lr != 0.f)) {
+        weights = 0.f;
+        for (int c = 0; c < cluster; ++c) weights += sh.teacher[xc][c].q;
+      }
+      const float inv_l = bad ? nan_f() : (l == 0.f ? 0.f : weights / l);
       const float coef = bad ? nan_f() : (lr == 0.f ? 0.f : share * inv_l - q_rest / lr);
       if (WRITE) {
         const float w = a.grad_scale / a.temperature;

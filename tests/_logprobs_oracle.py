@@ -127,6 +127,8 @@ def distill(x, values, ids, t, tail):
         g = p.clone()
         w = p.clone()
         q_rest, lift = 0.0, 0.0
+        # d(-sum w_k log p_k)/dx_j = (sum of the weights w_k in the loss) p_j - w_j
+        weights = float(q.sum()) if tail == "bucket" else 1.0
         outside = torch.ones(V, dtype=torch.bool)
         outside[col] = False
         if tail == "bucket":
@@ -137,12 +139,14 @@ def distill(x, values, ids, t, tail):
                 share = torch.exp(inside_rest - torch.logsumexp(inside_rest, 0))
                 if q_rest > 0:
                     total = total + q_rest * (math.log(q_rest) - log_rest)
+                    weights = 1.0
                     g -= q_rest * share
                 # 1 - sum q in 32 bits: off by 140 u, whatever is left of it
                 lift = 140 * U
                 size = size + q_rest * (abs(math.log(q_rest)) if q_rest > 0 else 0.0) + q_rest * abs(float(log_rest))
                 loss_off[i] += lift * (abs(float(log_rest)) + 18 + (abs(math.log(q_rest)) if q_rest > 0 else 0.0))
                 w += (q_rest + lift / r) * share
+        g += (weights - 1.0) * p
         g.scatter_add_(0, col, -q)
         w.scatter_add_(0, col, q)
         loss[i], grad[i] = total, g / t

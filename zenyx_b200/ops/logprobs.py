@@ -254,13 +254,15 @@ def _distill_torch(x, values, ids, temperature: float, bucket: bool):
     loss = torch.where(q == 0, 0.0, q * (q.log() - lp.gather(1, at))).sum(dim=1)
     grad = lp.exp()
     if bucket:
-        rest = (1.0 - q.sum(dim=1, keepdim=True)).clamp(min=0.0)
+        total = q.sum(dim=1, keepdim=True)
+        rest = (1.0 - total).clamp(min=0.0)
         inside = torch.zeros_like(x).scatter_add_(1, at, there.to(x.dtype)) > 0
         outside = lp.masked_fill(inside, _NEG)
         log_rest = torch.logsumexp(outside, dim=1, keepdim=True)
         some = (rest > 0) & (log_rest != _NEG)
         loss = loss + torch.where(some, rest * (rest.log() - log_rest), 0.0)[:, 0]
-        grad = grad - torch.where(some & (outside != _NEG), rest * (outside - log_rest).exp(), 0.0)
+        # the weights in the loss add up to 1, except where the remainder is not among them
+        grad = grad * torch.where(some, 1.0, total) - torch.where(some & (outside != _NEG), rest * (outside - log_rest).exp(), 0.0)
     grad = grad.scatter_add(1, at, -q) / temperature
     return loss.masked_fill(~live, 0.0), grad.masked_fill(~live[:, None], 0.0)
 
@@ -310,7 +312,8 @@ def distill_topk(logits: torch.Tensor, teacher_logprobs: torch.Tensor, teacher_i
     ``tail="renormalize"``: q = softmax(teacher_logprobs) over the K tokens (so logits do as well),
     sum_k q_k (log q_k - log p_k). ``tail="bucket"``: q = exp(teacher_logprobs), and all other tokens are one, with
     what is left of either distribution: + q_r (log q_r - log p_r), where q_r = max(0, 1 - sum_k q_k); it is left out
-    where the student has nothing outside the K tokens.
+    where the student has nothing outside the K tokens. Values in bf16 or fp16 may add up to more than 1 by their
+    rounding: the loss takes them as they are.
 
     Entries whose token lies outside [0, V) (-1) are absent, whatever their value; a row without entries (or, for
     ``renormalize``, with values of -inf only) is left out: loss and gradient 0. A token that is named twice gets

@@ -865,13 +865,12 @@ std::tuple<MaybeTensor, Tensor, MaybeTensor, MaybeTensor> token_logprobs(const T
 }
 
 struct DistillFn : public torch::autograd::Function<DistillFn> {
-  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& logits, const Tensor& values, const Tensor& ids,
+  // v, k: [rows, K], contiguous
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& logits, const Tensor& v, const Tensor& k,
                         double temperature, bool bucket) {
     at::AutoDispatchBelowADInplaceOrView below;
     const Tensor x = rows_of(logits);
     const auto f32 = x.options().dtype(torch::kFloat32);
-    const int64_t K = ids.size(-1);
-    const Tensor v = values.reshape({x.size(0), K}).contiguous(), k = ids.reshape({x.size(0), K}).contiguous();
     Tensor loss = at::empty(lead_of(logits), f32), stats = at::empty({x.size(0), 4}, f32);
     distill_topk(x, v, k, loss, stats, c10::nullopt, c10::nullopt, 1.0, temperature, bucket);
     ctx->save_for_backward({logits, v, k, stats});
@@ -895,7 +894,11 @@ struct DistillFn : public torch::autograd::Function<DistillFn> {
 Tensor distill_topk_loss(const Tensor& logits, const Tensor& values, const Tensor& ids, double temperature, const std::string& tail) {
   check_user_logits(logits, temperature);
   check_teacher(logits, values, ids, tail);
-  return DistillFn::apply(logits, values.detach(), ids, temperature, tail == "bucket");
+  // Views are made here, where they share the version counters of the caller's tensors (below the autograd keys they would
+  // not): a backward that has kept a teacher which was overwritten is an error instead of wrong.
+  const int64_t rows = logits.numel() / logits.size(-1), K = ids.size(-1);
+  return DistillFn::apply(logits, values.detach().reshape({rows, K}).contiguous(), ids.reshape({rows, K}).contiguous(), temperature,
+                          tail == "bucket");
 }
 // Losses [rows]; out, or the logits themselves, gets grad_scale times the gradient of their sum.
 Tensor distill_topk_fwd_bwd(const Tensor& logits, const Tensor& values, const Tensor& ids, double grad_scale, double temperature,

@@ -1,0 +1,52 @@
+"""The operators on rows of logits as autograd functions: the CPU form and the CUDA form notice, refuse and return the same."""
+import pytest
+import torch
+
+from zenyx_b200.ops.logprobs import distill_topk, token_logprobs
+
+both = pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+
+
+def _case(device, shape=(2, 3), V=50, K=4, ids=torch.int64, values=torch.float32):
+    gen = torch.Generator().manual_seed(0)
+    x = torch.randn(*shape, V, generator=gen)
+    y = torch.randint(0, V, shape, generator=gen)
+    v, k = torch.log_softmax(torch.randn(*shape, V, generator=gen), -1).topk(K)
+    return x.to(device), y.to(device), v.to(values).to(device), k.to(ids).to(device)
+
+
+@both
+@pytest.mark.parametrize("shape", [(6,), (2, 3)])
+@pytest.mark.parametrize("kind", [(torch.int64, torch.float32), (torch.int32, torch.bfloat16)])
+@pytest.mark.parametrize("which", ["teacher_ids", "teacher_logprobs"])
+def test_a_teacher_overwritten_before_the_backward_is_noticed(device, shape, kind, which):
+    x, _, v, k = _case(device, shape, ids=kind[0], values=kind[1])
+    x.requires_grad_(True)
+    for tail in ("renormalize", "bucket"):
+        loss = distill_topk(x, v, k, tail=tail)
+        (k if which == "teacher_ids" else v).zero_()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.sum().backward()
+
+
+@both
+def test_targets_overwritten_before_the_backward_are_noticed(device):
+    x, y, _, _ = _case(device)
+    x.requires_grad_(True)
+    out = token_logprobs(x, y)
+    y.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.logprobs.sum().backward()
+
+
+@both
+def test_a_teacher_that_had_to_be_copied_may_be_overwritten(device):
+    x, _, v, k = _case(device)
+    x.requires_grad_(True)
+    (want,) = torch.autograd.grad(distill_topk(x, v, k).sum(), x)
+    v2, k2 = v.transpose(0, 1).contiguous().transpose(0, 1), k.transpose(0, 1).contiguous().transpose(0, 1)
+    loss = distill_topk(x, v2, k2)
+    v2.zero_()
+    k2.zero_()
+    (got,) = torch.autograd.grad(loss.sum(), x)
+    assert torch.equal(got, want)

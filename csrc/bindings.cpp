@@ -1,6 +1,7 @@
 // Python bindings of the sm_100a kernels. Tensors are validated here; the kernels themselves see
 // raw pointers, the current CUDA stream and one process-wide Status word.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/VariableTypeUtils.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -545,6 +546,7 @@ void check_dlogits(const Tensor& d, const Tensor& x) {
               "d_logits must have the shape, type and device of the logits");
   TORCH_CHECK(d.size(1) == 1 || d.stride(1) == 1, "d_logits must have contiguous columns");
   TORCH_CHECK(d.size(0) <= 1 || d.stride(0) >= d.size(1), "the rows of d_logits share memory");
+  torch::autograd::check_inplace(d, d.requires_grad());     // no leaf that wants a gradient
   if (d.numel() == 0) return;
   const bool same = d.data_ptr() == x.data_ptr() && (d.size(0) == 1 || d.stride(0) == x.stride(0));
   TORCH_CHECK(same || apart(d, x),

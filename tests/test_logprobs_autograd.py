@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from zenyx_b200.ops.logprobs import distill_topk, token_logprobs
+from zenyx_b200.ops.logprobs import distill_topk, distill_topk_fwd_bwd_, token_logprobs
 
 both = pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
 
@@ -50,3 +50,22 @@ def test_a_teacher_that_had_to_be_copied_may_be_overwritten(device):
     k2.zero_()
     (got,) = torch.autograd.grad(loss.sum(), x)
     assert torch.equal(got, want)
+
+
+@both
+def test_leaves_that_want_a_gradient_are_not_overwritten(device):
+    x, _, v, k = _case(device, (6,))
+    leaf, kept = x.clone().requires_grad_(True), x.clone()
+    for write in (lambda: distill_topk_fwd_bwd_(leaf, v, k, 1.0), lambda: distill_topk_fwd_bwd_(leaf[:], v, k, 1.0),
+                  lambda: distill_topk_fwd_bwd_(x, v, k, 1.0, out=leaf)):
+        with pytest.raises(RuntimeError, match="leaf Variable that requires grad"):
+            write()
+    assert torch.equal(leaf, kept) and torch.equal(x, kept)
+    want = torch.empty_like(x)
+    loss = distill_topk_fwd_bwd_(x, v, k, 1.0, out=want)
+    with torch.no_grad():                       # what an optimizer may do
+        assert torch.equal(distill_topk_fwd_bwd_(leaf, v, k, 1.0), loss)
+    assert torch.equal(leaf, want)
+    inner = kept.clone().requires_grad_(True) * 1.0
+    out = distill_topk_fwd_bwd_(inner, v, k, 1.0)
+    assert torch.equal(out, loss) and not out.requires_grad and torch.equal(inner, want)

@@ -271,7 +271,8 @@ def distill_topk_fwd_bwd_(logits: torch.Tensor, teacher_logprobs: torch.Tensor, 
                           grad_scale: float, *, temperature: float = 1.0, tail: str = "renormalize",
                           out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Overwrites `logits` [rows, V] (or fills `out`, which leaves them alone) with grad_scale * d(sum of
-    losses)/d(logits); returns the per-row losses (fp32). What the losses are: see ``distill_topk``."""
+    losses)/d(logits); returns the per-row losses (fp32), without a gradient of their own. What the losses are: see
+    ``distill_topk``."""
     if logits.is_cuda:      # the extension checks the same
         return _ext.C().distill_topk_fwd_bwd(logits, teacher_logprobs, teacher_ids, grad_scale, temperature, tail, out)
     _check_logits(logits, temperature)
@@ -281,7 +282,7 @@ def distill_topk_fwd_bwd_(logits: torch.Tensor, teacher_logprobs: torch.Tensor, 
     out = logits if out is None else out
     if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
         raise ValueError("out has the shape, type and device of the logits")
-    loss, grad = _distill_torch(_wide(logits), teacher_logprobs, teacher_ids, temperature, tail == "bucket")
+    loss, grad = _distill_torch(_wide(logits.detach()), teacher_logprobs.detach(), teacher_ids, temperature, tail == "bucket")
     out.copy_(grad * grad_scale)
     return loss
 

@@ -700,7 +700,12 @@ void distill_topk(const Tensor& logits, const Tensor& values, const Tensor& ids,
 // ---- the same as users call them, with their checks and as autograd functions. In C++: a call for a few rows is mostly
 // host time. The Python forms in ops/logprobs.py check the same for CPU tensors. ----
 
+// Forward-mode derivatives: none of these has one, and the kernels would drop the tangent.
+void check_no_tangent(const char* name, const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), name, ": there is no forward-mode derivative");
+}
 void check_user_logits(const Tensor& x, double temperature) {
+  check_no_tangent("logits", x);
   TORCH_CHECK_TYPE(x.scalar_type() == torch::kBFloat16 || x.scalar_type() == torch::kFloat16 || x.scalar_type() == torch::kFloat32,
                    "logits are bf16, fp16 or fp32, not ", x.scalar_type());
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= zx::kHeadMaxVocab, "logits are [..., V] with 1 <= V <= ",
@@ -728,6 +733,7 @@ void check_teacher(const Tensor& logits, const Tensor& values, const Tensor& ids
   TORCH_CHECK_VALUE(values.sizes() == ids.sizes(), "teacher_logprobs have shape ", values.sizes(), ", teacher_ids ", ids.sizes());
   TORCH_CHECK_VALUE(values.device() == logits.device(), "teacher_logprobs are on ", values.device(), ", the logits on ", logits.device());
   TORCH_CHECK_VALUE(!values.requires_grad() || !at::GradMode::is_enabled(), "the teacher gets no gradient: detach teacher_logprobs");
+  check_no_tangent("teacher_logprobs", values);
 }
 
 // Gradients that have none of their own: an error when somebody asks for it, as torch.autograd's once_differentiable.

@@ -1,6 +1,7 @@
 """The operators on rows of logits as autograd functions: the CPU form and the CUDA form notice, refuse and return the same."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from zenyx_b200.ops.logprobs import distill_topk, distill_topk_fwd_bwd_, token_logprobs
 
@@ -69,3 +70,36 @@ def test_leaves_that_want_a_gradient_are_not_overwritten(device):
     inner = kept.clone().requires_grad_(True) * 1.0
     out = distill_topk_fwd_bwd_(inner, v, k, 1.0)
     assert torch.equal(out, loss) and not out.requires_grad and torch.equal(inner, want)
+
+
+@both
+@pytest.mark.parametrize("wants_grad", [False, True])
+def test_tangents_are_refused_and_not_dropped(device, wants_grad):
+    x, y, v, k = _case(device, (6,))
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x.clone().requires_grad_(wants_grad), torch.ones_like(x))
+        teacher = forward_ad.make_dual(v.clone(), torch.ones_like(v))
+        calls = [lambda: token_logprobs(dual, y, top_k=2), lambda: token_logprobs(dual), lambda: distill_topk(dual, v, k),
+                 lambda: distill_topk(x, teacher, k), lambda: distill_topk_fwd_bwd_(x.clone(), teacher, k, 1.0),
+                 lambda: distill_topk_fwd_bwd_(dual, v, k, 1.0, out=torch.empty_like(x))]
+        for call in calls:
+            with pytest.raises(NotImplementedError):
+                call()
+            with pytest.raises(NotImplementedError), torch.no_grad():
+                call()
+        token_logprobs(x, y)            # what has no tangent goes through
+        distill_topk(x, v, k)
+
+
+@both
+def test_function_transforms_are_refused(device):
+    x, y, v, k = _case(device, (6,))
+    for f in (lambda z: token_logprobs(z, y).logprobs.sum(), lambda z: token_logprobs(z).entropy.sum(),
+              lambda z: distill_topk(z, v, k).sum()):
+        with pytest.raises(RuntimeError):
+            torch.func.grad(f)(x)
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(f, (x,), (torch.ones_like(x),))
+    for f in (lambda z: token_logprobs(z).entropy, lambda z: distill_topk(z, v[0], k[0])):
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(f)(x)

@@ -17,12 +17,15 @@ Rows and values that stand for nothing:
 * a logit of -inf has probability 0 and is no alternative. Missing alternatives have token -1 and log-probability -inf;
 * a row whose logits are all -inf has log-probability -inf, entropy 0 and no gradient;
 * a row that holds +inf or NaN has NaN everywhere and no alternatives.
+
+Gradients are reverse-mode and of first order: tensors with forward-mode tangents and function transforms are refused.
 """
 from __future__ import annotations
 
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _ext
 
@@ -47,7 +50,13 @@ class TokenLogprobs(NamedTuple):
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
+def _check_no_tangent(name: str, t: torch.Tensor) -> None:
+    if forward_ad.unpack_dual(t).tangent is not None:
+        raise NotImplementedError(f"{name}: there is no forward-mode derivative")
+
+
 def _check_logits(logits: torch.Tensor, temperature: float) -> None:
+    _check_no_tangent("logits", logits)
     if logits.dtype not in _TYPES and (logits.is_cuda or logits.dtype != torch.float64):
         raise TypeError(f"logits are bf16, fp16 or fp32 (fp64 on the CPU), not {logits.dtype}")
     if logits.dim() < 1 or not 1 <= logits.shape[-1] <= MAX_VOCAB:
@@ -231,6 +240,7 @@ def _check_teacher(logits, values, ids, tail: str) -> None:
         raise ValueError(f"teacher_logprobs are on {values.device}, the logits on {logits.device}")
     if values.requires_grad and torch.is_grad_enabled():
         raise ValueError("the teacher gets no gradient: detach teacher_logprobs")
+    _check_no_tangent("teacher_logprobs", values)
 
 
 def _distill_torch(x, values, ids, temperature: float, bucket: bool):

@@ -101,6 +101,48 @@ def test_two_rows_by_hand():
     assert torch.allclose(out[0], want, rtol=0, atol=1e-6)
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("t", [1.0, 1.5])
+@pytest.mark.parametrize("V,K", [(9, 2), (1000, 40), (50257, 128)])
+def test_the_remainder_of_a_peaked_teacher(device, V, K, t):
+    """What the bucket has left is off by half a step where it is small, and by the roundings of a sum of 128 weights
+    (140 u, u = 2^-24) of at least a quarter, 560 u of itself, where it is not. So is its part of the gradient,
+    q_r p_j / p_r, on top of the bounds of the logits' own sums (_logprobs_oracle.py)."""
+    U = oracle.U
+    left = [0.9, 0.3, 0.26, 0.24, 0.1, 1e-2, 1e-3, 1e-4, 1e-5, 1e-6, 3e-7]
+    gen = torch.Generator().manual_seed(K)
+    T = len(left)
+    ids = torch.stack([torch.randperm(V, generator=gen)[:K] for _ in range(T)])
+    spread = torch.softmax(torch.randn(T, K, generator=gen, dtype=torch.float64), 1)
+    left = torch.tensor(left, dtype=torch.float64)[:, None]
+    values = torch.log(spread * (1 - left)).float()
+    # the student has learnt most of it: twice the teacher's remainder lies outside
+    z = torch.randn(T, V, generator=gen, dtype=torch.float64).scatter(1, ids, NEG)
+    z = (torch.log_softmax(z, 1) + torch.log(2 * left)).scatter(1, ids, values.double() + 0.3 * torch.randn(T, K, generator=gen))
+    x = (z * t).float()
+    a = x.double().requires_grad_(True)
+    ref = _loss(a, values, ids, t)
+    (grad,) = torch.autograd.grad(ref.sum(), a)
+    rest = 1 - values.double().exp().sum(1)
+    assert bool((rest > 2e-7).all())
+    lp = torch.log_softmax(x.double() / t, 1)
+    outside = lp.scatter(1, ids, NEG)
+    share = torch.softmax(outside, 1)
+    r = oracle.rel_sum(V)
+    rounding = 4 * r + 2.1 * U * 1.4427 * 2 * lp.abs() + 140 * U
+    inside = torch.zeros_like(lp).scatter(1, ids, values.double().exp())
+    off = ((lp.exp() + inside) * rounding + rest[:, None] * share * (rounding + 560 * U)) / t
+    loss = distill_topk_fwd_bwd_(x.to(device), values.to(device), ids.to(device), 1.0, temperature=t, tail="bucket",
+                                 out=(out := torch.empty(T, V, device=device)))
+    oracle.check(out, grad, off, "gradient")
+    terms = inside * (inside.clamp(min=1e-300).log().abs() + lp.abs() + 1)
+    log_rest = torch.logsumexp(outside, 1)
+    size = terms.sum(1) + rest * (rest.log().abs() + log_rest.abs())
+    # d(q_r (log q_r - log p_r)) = (log q_r + 1 - log p_r) dq_r
+    off = (4 * r + 140 * U) * size + 560 * U * rest * (rest.log().abs() + 1 + log_rest.abs())
+    oracle.check(loss, ref.detach(), off, "loss")
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("value_type,above", [(torch.bfloat16, 0.0), (torch.float16, 0.0), (torch.float32, 0.05), (torch.float32, -0.7)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])

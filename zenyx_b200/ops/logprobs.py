@@ -264,8 +264,8 @@ def _distill_torch(x, values, ids, temperature: float, bucket: bool):
     loss = torch.where(q == 0, 0.0, q * (q.log() - lp.gather(1, at))).sum(dim=1)
     grad = lp.exp()
     if bucket:
-        total = q.sum(dim=1, keepdim=True)
-        rest = (1.0 - total).clamp(min=0.0)
+        total = v.double().exp().sum(dim=1, keepdim=True)     # a peaked teacher leaves few digits of the remainder in 32 bits
+        rest, total = (1.0 - total).clamp(min=0.0).to(x.dtype), total.to(x.dtype)
         inside = torch.zeros_like(x).scatter_add_(1, at, there.to(x.dtype)) > 0
         outside = lp.masked_fill(inside, _NEG)
         log_rest = torch.logsumexp(outside, dim=1, keepdim=True)

@@ -2,8 +2,10 @@
 //   forward:   z_y - lse of a given token y, the entropy H = -sum p (z - lse), the k most likely tokens;
 //   backward:  d/dx_j = (1 / temperature) [ g ([j = y] - p_j) - h p_j (z_j - lse + H) + sum_k c_k ([j = i_k] - p_j) ].
 // Both are bound by the bytes of the logits, read once each way. With l = sum 2^d, s = sum 2^d d (d = rel2, rows.cuh):
-// z_j - lse = ln 2 (d_j - log2 l), H = ln 2 (log2 l - s / l), in which both terms are >= 0, so nothing cancels. (maximum, l)
-// is what the backward needs. Sums are held in 32 bits, the few scalars of a row are put together in 64.
+// z_j - lse = ln 2 (d_j - log2 l), H = ln 2 (log2 l - s / l). d of the maximum is not 0 but the rounding of its reference (2^-5 at
+// most), so both terms of H may be that far from their sign, and where one token has all the mass they cancel: H and z_j - lse
+// are off by what l and s are, relatively (2^-22 and more with V), and are held at 0, which they would pass. (maximum, l) is what
+// the backward needs. Sums are held in 32 bits, the few scalars of a row are put together in 64.
 //
 // Measured on a B200 that copies 6557 GB/s: forward 4096 x 128256 bf16 161 us (6.5 TB/s), with 20 alternatives 200, 64
 // 218, 128 243; one row 4.5 us, with 20 alternatives 7.6 (launch and the search's chain of barriers); 64 x 128256 fp32
@@ -487,8 +489,8 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(LogprobsArgs 
       a.stats[(size_t)r * 2] = b.m;
       a.stats[(size_t)r * 2 + 1] = bad ? nan_f() : b.l;
     }
-    a.entropy[r] = bad ? nan_f() : (empty ? 0.f : (float)(log_l - kLn2 * (double)b.s / (double)b.l));
-    if (y >= 0) a.logprobs[r] = bad ? nan_f() : (empty ? -inf_f() : (float)(kLn2 * rel2_exact(xy, b.m, c2) - log_l));
+    a.entropy[r] = bad ? nan_f() : (empty ? 0.f : fmaxf((float)(log_l - kLn2 * (double)b.s / (double)b.l), 0.f));
+    if (y >= 0) a.logprobs[r] = bad ? nan_f() : (empty ? -inf_f() : fminf((float)(kLn2 * rel2_exact(xy, b.m, c2) - log_l), 0.f));
   };
   if (cluster > 1) cluster_wait();   // every block of the cluster has started: its shared memory may be written
   // The last warp's: joins the block's sums.
@@ -604,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(LogprobsArgs 
     const uint64_t key = bad ? 0 : top.best[k];
     a.top_ids[(size_t)r * K + k] = key == 0 ? -1 : (int64_t)alt_col(key);
     a.top_logprobs[(size_t)r * K + k] =
-        bad ? nan_f() : (key == 0 ? -inf_f() : (float)(kLn2 * rel2_exact(key_value((uint32_t)(key >> 32)), sh.m, c2) - sh.log_l));
+        bad ? nan_f() : (key == 0 ? -inf_f() : fminf((float)(kLn2 * rel2_exact(key_value((uint32_t)(key >> 32)), sh.m, c2) - sh.log_l), 0.f));
   }
 }
 

@@ -1,0 +1,27 @@
+"""Results of the operators on rows of logits lie where their definitions put them, and calls at the ends of what is allowed."""
+import pytest
+import torch
+
+from zenyx_b200.ops.logprobs import token_logprobs
+
+both = pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+dtypes = pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+
+
+@both
+@dtypes
+@pytest.mark.parametrize("V", [2, 300, 9001])
+def test_no_entropy_below_nothing_and_no_probability_above_one(device, dtype, V):
+    """One token with all of the mass, near zero and far from it, where roundings would pass the end of the range."""
+    gen = torch.Generator().manual_seed(V)
+    T = 400
+    size = torch.exp(torch.rand(T, generator=gen) * 13 + 1).clamp(max=6e4 if dtype == torch.float16 else 7e5)
+    sign = torch.where(torch.rand(T, generator=gen) < 0.5, -1.0, 1.0)
+    y = torch.randint(0, V, (T,), generator=gen)
+    x = (torch.randn(T, V, generator=gen) - 200 + (sign * size)[:, None]).clamp(min=-6e4 if dtype == torch.float16 else -8e5)
+    x.scatter_(1, y[:, None], (sign * size)[:, None])
+    x, y = x.to(dtype).to(device), y.to(device)
+    for t in (1.0, 0.7, 3.0):
+        out = token_logprobs(x, y, top_k=2, temperature=t)
+        assert bool((out.entropy >= 0).all()) and bool((out.logprobs <= 0).all()) and bool((out.top_logprobs <= 0).all())
+        assert bool((out.logprobs.exp() <= 1).all())

@@ -4,6 +4,7 @@
 #include <torch/csrc/autograd/VariableTypeUtils.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include "attn/attn.h"
@@ -759,43 +760,22 @@ std::vector<int64_t> lead_of(const Tensor& logits) {
 struct Scored {
   Tensor logprobs, entropy, stats, top, ids;    // undefined: not asked for
 };
-// Contiguous results on one device. Small ones lie in one allocation, 16 bytes apart: each allocation costs the host 0.8 us,
-// and the allocator gives out 512 bytes at least.
-class Results {
- public:
-  Results(c10::Device device, int64_t bytes) : device_(device) {
-    if (bytes <= 4096) shared_ = at::empty({bytes}, at::TensorOptions().dtype(torch::kUInt8).device(device));
-  }
-  static int64_t bytes_for(int64_t n, int64_t each) { return (n * each + 15) / 16 * 16; }
-  Tensor take(c10::IntArrayRef sizes, torch::ScalarType type) {
-    if (!shared_.defined()) return at::empty(sizes, at::TensorOptions().dtype(type).device(device_));
-    const int64_t each = c10::elementSize(type), n = c10::multiply_integers(sizes);
-    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(shared_.storage()), shared_.key_set(), c10::scalarTypeToTypeMeta(type));
-    t.unsafeGetTensorImpl()->set_storage_offset(used_ / each);
-    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
-    used_ += bytes_for(n, each);
-    return t;
-  }
-
- private:
-  c10::Device device_;
-  Tensor shared_;
-  int64_t used_ = 0;
-};
+// A result: without the dispatcher, since the allocations of a call for a few rows are a third of its host time.
+Tensor result(c10::IntArrayRef sizes, torch::ScalarType type, c10::Device device) {
+  return at::detail::empty_cuda(sizes, type, device, c10::nullopt);
+}
 Scored score(const Tensor& logits, const Tensor& targets, int64_t top_k, double temperature, bool with_stats) {
   const Tensor x = rows_of(logits);
   auto lead = lead_of(logits);
   const int64_t rows = x.size(0);
-  Results results(x.device(), Results::bytes_for(rows, 4) * (targets.defined() ? 2 : 1) + (with_stats ? Results::bytes_for(rows, 8) : 0) +
-                                  Results::bytes_for(rows * top_k, 4) + Results::bytes_for(rows * top_k, 8));
   Scored o;
-  o.entropy = results.take(lead, torch::kFloat32);
-  if (targets.defined()) o.logprobs = results.take(lead, torch::kFloat32);
-  if (with_stats) o.stats = results.take({rows, 2}, torch::kFloat32);
+  o.entropy = result(lead, torch::kFloat32, x.device());
+  if (targets.defined()) o.logprobs = result(lead, torch::kFloat32, x.device());
+  if (with_stats) o.stats = result({rows, 2}, torch::kFloat32, x.device());
   if (top_k > 0) {
     lead.push_back(top_k);
-    o.top = results.take(lead, torch::kFloat32);
-    o.ids = results.take(lead, torch::kInt64);
+    o.top = result(lead, torch::kFloat32, x.device());
+    o.ids = result(lead, torch::kInt64, x.device());
   }
   auto opt = [](const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; };
   auto flat = [&](const Tensor& t) {

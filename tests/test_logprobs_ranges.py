@@ -1,4 +1,6 @@
 """Results of the operators on rows of logits lie where their definitions put them, and calls at the ends of what is allowed."""
+import io
+
 import pytest
 import torch
 
@@ -25,3 +27,19 @@ def test_no_entropy_below_nothing_and_no_probability_above_one(device, dtype, V)
         out = token_logprobs(x, y, top_k=2, temperature=t)
         assert bool((out.entropy >= 0).all()) and bool((out.logprobs <= 0).all()) and bool((out.top_logprobs <= 0).all())
         assert bool((out.logprobs.exp() <= 1).all())
+
+
+@both
+@pytest.mark.parametrize("T", [1, 3, 4000])
+def test_results_have_storages_of_their_own(device, T):
+    """What is written to a file is the result and no more, whatever the size of the call."""
+    x = torch.randn(T, 60, device=device)
+    y = torch.randint(0, 60, (T,), device=device)
+    for wants_grad in (False, True):
+        out = token_logprobs(x.clone().requires_grad_(wants_grad), y, top_k=2)
+        assert len({t.untyped_storage().data_ptr() for t in out}) == 4
+        for t in out:
+            assert t.storage_offset() == 0 and t.untyped_storage().nbytes() == t.numel() * t.element_size()
+            file = io.BytesIO()
+            torch.save(t.detach(), file)
+            assert file.tell() < t.numel() * t.element_size() + 2048

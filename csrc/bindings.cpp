@@ -1,6 +1,7 @@
 // Python bindings of the sm_100a kernels. Tensors are validated here; the kernels themselves see
 // raw pointers, the current CUDA stream and one process-wide Status word.
 #include <torch/extension.h>
+#include <atomic>
 #include <torch/csrc/autograd/VariableTypeUtils.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <ATen/cuda/CUDAContext.h>
@@ -785,6 +786,10 @@ Scored score(const Tensor& logits, const Tensor& targets, int64_t top_k, double 
   return o;
 }
 
+// Kernels launched by backward passes, which no call of the extension stands for.
+std::atomic<int64_t> g_autograd_launches{0};
+int64_t autograd_launches() { return g_autograd_launches.load(); }
+
 struct TokenLogprobsFn : public torch::autograd::Function<TokenLogprobsFn> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits,
                                                 const c10::optional<Tensor>& targets, int64_t top_k, double temperature) {
@@ -819,6 +824,7 @@ struct TokenLogprobsFn : public torch::autograd::Function<TokenLogprobsFn> {
       token_logprobs_bwd(x, y.defined() ? c10::optional<Tensor>(y) : c10::nullopt, entropy, stats,
                          top_k > 0 ? c10::optional<Tensor>(ids.view({x.size(0), top_k})) : c10::nullopt, fp32_rows(d_lp),
                          fp32_rows(d_entropy), fp32_rows(d_top), d2, ctx->saved_data["temperature"].toDouble());
+      ++g_autograd_launches;
     }
     return {d.defined() ? differentiable_once(d) : d, Tensor(), Tensor(), Tensor()};
   }
@@ -875,6 +881,7 @@ struct DistillFn : public torch::autograd::Function<DistillFn> {
       d = at::empty(saved[0].sizes(), x.options());
       distill_topk(x, saved[1], saved[2], c10::nullopt, saved[3], fp32_rows(grads[0]), d.view({x.size(0), x.size(1)}), 1.0,
                    ctx->saved_data["temperature"].toDouble(), ctx->saved_data["bucket"].toBool());
+      ++g_autograd_launches;
     }
     return {differentiable_once(d), Tensor(), Tensor(), Tensor(), Tensor()};
   }
@@ -907,6 +914,7 @@ Tensor distill_topk_fwd_bwd(const Tensor& logits, const Tensor& values, const Te
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  m.def("autograd_launches", &autograd_launches);
   m.def("read_status", &read_status, "read (and optionally clear) the kernel status word");
   m.def("gemm", &gemm, py::arg("a"), py::arg("b"), py::arg("out"), py::arg("a_t"), py::arg("b_t"), py::arg("addend"),
         py::arg("pull_src") = 0, py::arg("pull_dst") = 0, py::arg("pull_bytes") = 0,

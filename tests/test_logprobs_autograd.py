@@ -103,3 +103,17 @@ def test_function_transforms_are_refused(device):
     for f in (lambda z: token_logprobs(z).entropy, lambda z: distill_topk(z, v[0], k[0])):
         with pytest.raises(RuntimeError):
             torch.func.vmap(f)(x)
+
+
+@pytest.mark.gpu
+def test_kernels_of_a_backward_pass_are_counted():
+    from zenyx_b200.ops import _ext
+
+    x, y, v, k = _case("cuda")
+    x.requires_grad_(True)
+    start = _ext.launch_count
+    out, loss = token_logprobs(x, y, top_k=2), distill_topk(x, v, k)
+    assert _ext.launch_count == start + 2
+    out.entropy.sum().backward()
+    loss.sum().backward()
+    assert _ext.launch_count == start + 4

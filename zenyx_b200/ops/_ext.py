@@ -45,7 +45,14 @@ def _load(name: str):
 # Kernel launches issued per binding call (everything else launches exactly one kernel).
 _LAUNCHES = {"attn_bwd": 3, "read_status": 0, "peer_alloc": 0, "peer_export": 0, "peer_open": 0, "peer_close": 0,
              "peer_free": 0, "tensor_from_ptr": 0}
-launch_count = 0
+_calls_launched = 0
+
+
+def __getattr__(name):
+    if name == "launch_count":      # of this process: by calls of the extension, and by its autograd functions' backward passes
+        mod = _mods.get("_C")
+        return _calls_launched + (mod.autograd_launches() if mod is not None else 0)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 class _CountingProxy:
@@ -62,8 +69,8 @@ class _CountingProxy:
             n = _LAUNCHES.get(name, 1)
 
             def fn(*args, __raw=raw, __n=n, **kwargs):
-                global launch_count
-                launch_count += __n
+                global _calls_launched
+                _calls_launched += __n
                 return __raw(*args, **kwargs)
 
             self._cache[name] = fn

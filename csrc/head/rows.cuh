@@ -12,6 +12,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <float.h>
+#include <algorithm>
 #include "../common/ptx.cuh"
 #include "logprobs.h"
 
@@ -360,7 +361,8 @@ int most_vecs(const void* p, int64_t ld, int rows, int V) {
 template <class... P, class... A>
 void launch(void (*kernel)(P...), int rows, int blocks_a_row, bool cluster, int threads, int smem, cudaStream_t st, A... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)rows * (unsigned)blocks_a_row);
+  // (a grid holds 2^31 - 1 blocks: a launch of more is refused)
+  cfg.gridDim = dim3((unsigned)std::min<int64_t>((int64_t)rows * blocks_a_row, UINT32_MAX));
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;

@@ -43,3 +43,13 @@ def test_results_have_storages_of_their_own(device, T):
             file = io.BytesIO()
             torch.save(t.detach(), file)
             assert file.tell() < t.numel() * t.element_size() + 2048
+
+
+@pytest.mark.gpu
+def test_more_blocks_than_a_grid_holds_are_refused():
+    """2^30 + 1 rows (one row, many times) of a vocabulary that takes four blocks a row."""
+    x = torch.zeros(1, 400000, device="cuda").expand((1 << 30) + 1, 400000)
+    with pytest.raises(RuntimeError, match="launch failed"):
+        token_logprobs(x)
+    torch.cuda.synchronize()
+    assert float(token_logprobs(x[:3]).entropy.max()) > 12      # nothing is left behind

@@ -4,7 +4,7 @@ import io
 import pytest
 import torch
 
-from zenyx_b200.ops.logprobs import token_logprobs
+from zenyx_b200.ops.logprobs import distill_topk_fwd_bwd_, token_logprobs
 
 both = pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
 dtypes = pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
@@ -53,3 +53,45 @@ def test_more_blocks_than_a_grid_holds_are_refused():
         token_logprobs(x)
     torch.cuda.synchronize()
     assert float(token_logprobs(x[:3]).entropy.max()) > 12      # nothing is left behind
+
+
+@both
+@dtypes
+@pytest.mark.parametrize("V,gap", [(100, 0), (101, 3), (50257, 1)])
+def test_logits_and_gradient_side_by_side(device, dtype, V, gap):
+    """Rows of one buffer: the logits in their first columns, the gradient behind them, and the other way round."""
+    T = 5
+    x = (torch.randn(T, V, device=device) * 2).to(dtype)
+    ids = torch.randint(0, V, (T, 3), device=device)
+    values = torch.full((T, 3), -2.0, device=device)
+    want = torch.empty_like(x)
+    loss = distill_topk_fwd_bwd_(x.clone(), values, ids, 1.0, out=want)
+    for logits_first in (True, False):
+        buffer = torch.full((T, 2 * V + gap + 5), 9.0, device=device, dtype=dtype)
+        a, b = buffer[:, :V], buffer[:, V + gap: 2 * V + gap]
+        logits, out = (a, b) if logits_first else (b, a)
+        logits.copy_(x)
+        got = distill_topk_fwd_bwd_(logits, values, ids, 1.0, out=out)
+        assert torch.equal(logits, x) and bool((buffer[:, 2 * V + gap:] == 9).all()) and bool((buffer[:, V: V + gap] == 9).all())
+        # rows at other addresses are summed up in another order: V / 128 + 16 roundings along the longest chain, twice
+        rel = 2 * (V / 128 + 16) * 2.0 ** -24 + 2.0 ** -20
+        assert bool(((got - loss).abs() <= rel * (1 + loss.abs())).all())
+        off = (out.float() - want.float()).abs()
+        assert bool((off <= (want.float().abs() + 0.5) * rel + want.float().abs() * torch.finfo(dtype).eps).all())
+
+
+@pytest.mark.gpu
+def test_gradients_that_cross_the_logits_are_refused():
+    flat = torch.zeros(5 * 220, device="cuda")
+    ids, values = torch.zeros(3, 2, device="cuda", dtype=torch.int64), torch.zeros(3, 2, device="cuda")
+
+    def rows(first):
+        return flat.as_strided((3, 100), (220, 1), first)
+
+    for first in (110 - 99, 110 + 1, 110 + 99, 110 + 121, 110 + 220):     # the last two reach the next row's logits
+        with pytest.raises(RuntimeError, match="overlaps"):
+            distill_topk_fwd_bwd_(rows(110), values, ids, 1.0, out=rows(first))
+    for first in (110 - 100, 110 + 100, 110 + 120):
+        distill_topk_fwd_bwd_(rows(110), values, ids, 1.0, out=rows(first))
+    with pytest.raises(RuntimeError, match="overlaps"):                    # rows at another distance
+        distill_topk_fwd_bwd_(rows(110), values, ids, 1.0, out=flat.as_strided((3, 100), (230, 1), 210))

@@ -59,3 +59,46 @@ def test_scores_over_a_ring_are_a_single_processs(tmp_path, world, layout):
         clear = ((best[..., :-1] - best[..., 1:]) > 2 * d).all(-1) & live
         assert float(clear.float().sum()) > 0.5 * float(live.float().sum())
         assert torch.equal(ids[clear], cut(want.top_ids)[clear])
+
+
+class _Peer:
+    """A ring's buffers as the model's host code sees them (the CPU's ring does not use them)."""
+
+    def __init__(self, sequences):
+        self.kv_shape = (sequences, S, 1, 32)
+
+
+@pytest.mark.parametrize("sequences", [1, 2, 3])
+def test_more_sequences_than_the_rings_buffers_hold(monkeypatch, sequences):
+    model = _model()
+    gen = torch.Generator().manual_seed(2)
+    tokens = torch.randint(0, V, (5, S), generator=gen)
+    want = model.token_logprobs(tokens, tokens, top_k=2)
+    seen, layer = [], model._layer_forward
+    monkeypatch.setattr(model, "_layer_forward", lambda l, h, B, *a, **kw: (seen.append(B), layer(l, h, B, *a, **kw))[1])
+    ring = RingContext(rank=0, degree=1, seq_len=S, peer=_Peer(sequences))
+    got = model.token_logprobs(tokens, tokens, top_k=2, ring=ring)
+    assert max(seen) == sequences and sum(seen) == 5 * model.cfg.n_layers
+    assert torch.equal(got.top_ids, want.top_ids) and torch.allclose(got.logprobs, want.logprobs, rtol=0, atol=1e-4)
+    assert model.logits(tokens, ring).shape == (5, S, V)
+
+
+def test_views_of_a_ring_slot_stay_inside_it():
+    """One more sequence than the slot holds would lay K across V."""
+    from zenyx_b200.parallel.peer import RingBuffers
+
+    class Memory:
+        def tensor(self, rank, offset, shape, dtype):
+            return offset, shape
+
+    ring = object.__new__(RingBuffers)
+    ring.kv_shape, ring.n, ring.fp8_block_tokens, ring.dtype = (2, 8, 1, 4), 64, 0, torch.bfloat16
+    ring.kv_bytes, ring.slot_bytes, ring.dkv_bytes = 128, 256, 256
+    ring.staging, ring.kv, ring.dkv = torch.arange(256.0).view(2, 2, 64), Memory(), Memory()
+    assert ring.kv_views(0, 1) == ((256, (2, 8, 1, 4)), (384, (2, 8, 1, 4)))
+    assert ring.kv_views(0, 0, (1, 8, 1, 4))[1] == (128, (1, 8, 1, 4))
+    k, v = ring.staged_kv(1, (1, 8, 1, 4))
+    assert torch.equal(k.reshape(-1), torch.arange(128.0, 160)) and torch.equal(v.reshape(-1), torch.arange(192.0, 224))
+    for bad in (lambda: ring.kv_views(0, 0, (3, 8, 1, 4)), lambda: ring.staged_kv(0, (3, 8, 1, 4)), lambda: ring.dkv_views(0, 0, (2, 9, 1, 4))):
+        with pytest.raises(ValueError):
+            bad()

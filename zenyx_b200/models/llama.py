@@ -515,9 +515,13 @@ class LlamaModel(nn.Module):
         return loss
 
     def forward(self, tokens: torch.Tensor, ring: Optional[RingContext] = None) -> torch.Tensor:
-        """Hidden states after the final norm, [B, S_local, d_model] (no gradient tracking)."""
+        """Hidden states after the final norm, [B, S_local, d_model] (no gradient tracking). Over a ring the sequences go
+        as many at a time as its K/V buffers were made for."""
         B, S = tokens.shape
         ring = self._ring(ring, S)
+        most = ring.peer.kv_shape[0] if ring.peer is not None else B
+        if B > most:
+            return torch.cat([self.forward(tokens[b: b + most], ring) for b in range(0, B, most)])
         with torch.no_grad():
             h = fused.embedding_fwd(tokens, self.w("embed.weight"))
             for l in range(self.cfg.n_layers):

@@ -10,6 +10,7 @@ zenyx/distributed/communication.py:136-171).
 from __future__ import annotations
 
 import itertools
+import math
 from typing import List, Optional, Sequence, Tuple
 
 import torch
@@ -180,16 +181,23 @@ class RingBuffers:
         return self._dequant(*self._q_layout(view))
 
     # K/V slot views -------------------------------------------------------------------------
+    def _shape(self, shape) -> Tuple[int, ...]:
+        shape = tuple(shape or self.kv_shape)
+        if math.prod(shape) > self.n:       # K would run into V, and V into the next slot
+            raise ValueError(f"K/V of shape {shape} exceed the ring's buffers, which were made for {self.kv_shape}")
+        return shape
+
     def kv_views(self, rank: int, slot: int, shape=None) -> Tuple[torch.Tensor, torch.Tensor]:
         assert self.fp8_block_tokens == 0, "e4m3 slots hold codes: use quantize_into_slot / dequant_*"
-        shape = tuple(shape or self.kv_shape)
+        shape = self._shape(shape)
         base = slot * self.slot_bytes
         return (self.kv.tensor(rank, base, shape, self.dtype),
                 self.kv.tensor(rank, base + self.kv_bytes, shape, self.dtype))
 
     def staged_kv(self, idx: int, shape=None) -> Tuple[torch.Tensor, torch.Tensor]:
-        shape = tuple(shape or self.kv_shape)
-        return self.staging[idx, 0].view(shape), self.staging[idx, 1].view(shape)
+        shape = self._shape(shape)
+        n = math.prod(shape)
+        return self.staging[idx, 0][:n].view(shape), self.staging[idx, 1][:n].view(shape)
 
     def pull_args(self, owner: int, slot: int, stage: int) -> Tuple[int, int, int]:
         """(src, dst, nbytes) copying owner's slot (K and V, in e4m3 mode also their scales, are adjacent) into
@@ -205,7 +213,7 @@ class RingBuffers:
 
     # dK/dV accumulators ---------------------------------------------------------------------
     def dkv_views(self, rank: int, slot: int, shape=None) -> Tuple[torch.Tensor, torch.Tensor]:
-        shape = tuple(shape or self.kv_shape)
+        shape = self._shape(shape)
         base = slot * 2 * self.dkv_bytes
         return (self.dkv.tensor(rank, base, shape, torch.float32),
                 self.dkv.tensor(rank, base + self.dkv_bytes, shape, torch.float32))

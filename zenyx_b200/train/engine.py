@@ -137,15 +137,16 @@ class LlamaEngine:
 
     def distill_step(self, tokens: torch.Tensor, teacher_logprobs: torch.Tensor, teacher_ids: torch.Tensor,
                      lr: Optional[float] = None, presharded: bool = False, *, temperature: float = 1.0,
-                     tail: str = "renormalize") -> torch.Tensor:
+                     tail: str = "renormalize", loss_scale: float = 1.0) -> torch.Tensor:
         """``train_step`` on what a teacher wrote down for the same tokens ([global_batch, seq_len, K] each, see
-        ``LlamaModel.forward_backward_distill``)."""
+        ``LlamaModel.forward_backward_distill``). Loss and gradients are ``loss_scale`` times the mean over all tokens'."""
         if not presharded:
             tokens = self.shard_batch(tokens)
             teacher_logprobs, teacher_ids = self.shard_batch(teacher_logprobs), self.shard_batch(teacher_ids)
         ring = self.ring
         return self._step(tokens, lr, lambda i, weight: self.model.forward_backward_distill(
-            tokens[i: i + 1], teacher_logprobs[i: i + 1], teacher_ids[i: i + 1], weight, ring, temperature=temperature, tail=tail))
+            tokens[i: i + 1], teacher_logprobs[i: i + 1], teacher_ids[i: i + 1], weight * loss_scale, ring, temperature=temperature,
+            tail=tail))
 
     def _step(self, tokens: torch.Tensor, lr: Optional[float], micro_batch) -> torch.Tensor:
         loss_weight = 1.0 / (self.cfg.global_batch * self.cfg.seq_len)

@@ -127,14 +127,16 @@ class Trainer:
         return float(reduced.item() / get_world_size())
 
     def distill_step(self, tokens: torch.Tensor, teacher_logprobs: torch.Tensor, teacher_ids: torch.Tensor, *,
-                     temperature: float = 1.0, tail: str = "renormalize") -> float:
+                     temperature: float = 1.0, tail: str = "renormalize", loss_scale: float = 1.0) -> float:
         """One optimizer step of the flagship on what a teacher wrote down for the same tokens: ``teacher_logprobs`` and
-        ``teacher_ids`` [global_batch, seq_len, K] from ``LlamaModel.token_logprobs(top_k=K)``. Returns the global mean
-        divergence (positions that the teacher left out count as 0). What the loss is: ``ops.logprobs.distill_topk``."""
+        ``teacher_ids`` [global_batch, seq_len, K] from ``LlamaModel.token_logprobs(top_k=K)``. Returns ``loss_scale`` times
+        the global mean divergence (positions that the teacher left out count as 0), which is what the step descends:
+        temperature^2, as softened targets are usually weighted, or tokens / positions that count for a mean over those.
+        What the loss is: ``ops.logprobs.distill_topk``."""
         if self.engine is None:
             raise ValueError("distill_step needs the flagship path: Trainer(LlamaConfig, ...)")
         return self._engine_step(lambda: self.engine.distill_step(tokens, teacher_logprobs, teacher_ids, lr=self._lr(),
-                                                                  temperature=temperature, tail=tail))
+                                                                  temperature=temperature, tail=tail, loss_scale=loss_scale))
 
     def _engine_step(self, step: Callable[[], torch.Tensor]) -> float:
         cur = self.config.curriculum

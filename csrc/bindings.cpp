@@ -613,7 +613,6 @@ void token_logprobs_fwd(const Tensor& logits, const c10::optional<Tensor>& targe
     a.top_logprobs = const_cast<float*>(float_rows(top_logprobs, (int64_t)a.rows * a.top_k, logits, "top_logprobs"));
   }
   c10::cuda::CUDAGuard guard(logits.device());
-  a.status = status_ptr();
   a.sm_count = sm_count();
   a.stream = cur_stream();
   zx::launch_token_logprobs_fwd(a);
@@ -647,7 +646,6 @@ void token_logprobs_bwd(const Tensor& logits, const c10::optional<Tensor>& targe
   a.d_logits = d_logits.data_ptr();
   a.d_ld = d_logits.stride(0);
   c10::cuda::CUDAGuard guard(logits.device());
-  a.status = status_ptr();
   a.sm_count = sm_count();
   a.stream = cur_stream();
   zx::launch_token_logprobs_bwd(a);

@@ -493,7 +493,6 @@ __global__ void __launch_bounds__(kWorkers + 32, 6) distill_kernel(DistillArgs a
   if (warp == kWorkerWarps) {
     distill_auxiliary<T>(a, sh, stage, cluster, rank, c2);
   } else {
-    const uint64_t c22 = pair(c2, c2);
     // The worker warps go their own ways: what they need of one another they get through the exchange.
     for (int n = 0, live_rows = 0;; ++n) {
       bool ok = mbar_wait_w(&sh.ready, n & 1, &sh.abort);

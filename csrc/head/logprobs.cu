@@ -354,8 +354,9 @@ __device__ __forceinline__ void add_group(const uint4 (&v)[U], float M, float c2
 // help either (ties, large logits side by side), the k are selected by their digits from all of the row.
 // What the search costs is its chain of barriers and reads, in which a block asks for little: 7 us of a row's 29 at 4096 x
 // 128256. Of the 13,800 clocks that one row with 20 alternatives takes, 3500 are the scan, 1300 sums and bound, 550 the list
-// of groups, 2000 the second look, 1200 the order, 1200 the exchange in the cluster, 2500 the merge. Copies into shared memory ahead of their use (a ring for each warp) made it 242 us instead of 219, larger steps
-// 240, the next row's start in the L2 cache 227.
+// of groups, 2000 the second look, 1200 the order, 1200 the exchange in the cluster, 2500 the merge. Copies into shared
+// memory ahead of their use (a ring for each warp) made it 242 us instead of 219, larger steps 240, the next row's start in the
+// L2 cache 227.
 template <class T, bool TOP>
 __global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(LogprobsArgs a, int cluster, int steps) {
   // TOP: TopShared, the keys of the cluster's blocks [cluster][k] (in the first block), the group maxima
@@ -605,8 +606,8 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(LogprobsArgs 
   for (int k = tid; k < K; k += nt) {
     const uint64_t key = bad ? 0 : top.best[k];
     a.top_ids[(size_t)r * K + k] = key == 0 ? -1 : (int64_t)alt_col(key);
-    a.top_logprobs[(size_t)r * K + k] =
-        bad ? nan_f() : (key == 0 ? -inf_f() : fminf((float)(kLn2 * rel2_exact(key_value((uint32_t)(key >> 32)), sh.m, c2) - sh.log_l), 0.f));
+    const double lp = kLn2 * rel2_exact(key_value((uint32_t)(key >> 32)), sh.m, c2) - sh.log_l;
+    a.top_logprobs[(size_t)r * K + k] = bad ? nan_f() : (key == 0 ? -inf_f() : fminf((float)lp, 0.f));
   }
 }
 

@@ -40,7 +40,6 @@ struct LogprobsArgs {
   const float* d_top = nullptr;        // [rows, top_k] or null
   void* d_logits = nullptr;
   int64_t d_ld = 0;
-  Status* status = nullptr;
   int sm_count = 0;
   cudaStream_t stream = nullptr;
 };

@@ -166,19 +166,6 @@ struct Vec {
       return __uint_as_float(w);
     }
   }
-  // element e becomes -inf where bit e of mask is set
-  static __device__ __forceinline__ void drop(uint4& v, uint32_t mask) {
-    uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (Elem<T>::kPerWord == 2) {
-        const uint32_t m = ((mask >> (2 * i) & 1) ? 0xffffu : 0u) | ((mask >> (2 * i + 1) & 1) ? 0xffff0000u : 0u);
-        w[i] = (w[i] & ~m) | (Elem<T>::kNegInf & m);
-      } else {
-        if (mask >> i & 1) w[i] = Elem<T>::kNegInf;
-      }
-    }
-  }
   static __device__ __forceinline__ uint4 nothing() {
     return make_uint4(Elem<T>::kNegInf, Elem<T>::kNegInf, Elem<T>::kNegInf, Elem<T>::kNegInf);
   }

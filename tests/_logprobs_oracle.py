@@ -4,9 +4,11 @@ Tolerances (u = 2^-24, half a step of fp32; t_out = eps(type) / 2, half a step o
 
 * an exponential 2^d is off by 2^-22 of itself (the hardware's, with a margin of two), and its argument
   d = (x - m) log2(e) / t by 3 u |d| (a subtraction, a product, the factor's own rounding): relative 3 u ln 2 |d| < 2.1 u |d|;
-* a sum of V exponentials adds one rounding a term along the longest chain, ceil(V / 128) + 16 (no row has fewer
-  than 128 threads, and a tree joins them): l is off by rel(V) = (ceil(V / 128) + 16) u + 2^-22 + 2.1 u <|d|> where
-  <|d|>, the mean over the distribution, is at most log2(V) plus a few: 32 covers V <= 2^20.
+* a sum of V exponentials adds one rounding a term along the longest chain, ceil(V / 128) + 16: a row of up to 128 vectors of
+  16 bytes has a thread for each of them (eight terms at most, four sums of two), a longer one 128 threads or more, and a
+  tree joins a thread's sums (2), the warp (5), the block (3) and the cluster (3). l is off by
+  rel(V) = (ceil(V / 128) + 16) u + 2^-22 + 2.1 u <|d|> where <|d|>, the mean over the distribution, is at most log2(V) plus
+  a few: 32 covers V <= 2^20.
   logprob = (x - m) / t - ln l: rel(V) plus the rounding of the result, u |logprob|;
 * the entropy's second sum has terms 2^d d of one sign: <|d|> times the same relative error, and one product more;
 * p is off by 2 rel(V) + 2.1 u |d| of itself; gradients add at most one more rounding for each of the at most 260

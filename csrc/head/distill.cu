@@ -6,8 +6,9 @@
 // where s is the sum of the weights in the loss: 1, but sum q where a bucket has nothing left (rounded values may add up to
 // more than 1) or where the student has nothing outside, so that the bucket's part is not in the loss.
 // Bound by the bytes of the logits, read once, and of the gradient. Measured on a B200 that copies 6557 GB/s, 64 of the
-// teacher's tokens: loss and gradient of 4096 x 128256 bf16 391 us (5.4 TB/s), 4096 x 32000 fp32 168 (6.2), 4000 x 50257
-// bf16 161 (5.0), 256 x 512 7.0 us; the loss alone of 4096 x 128256 227 us (4.6), its gradient from the statistics 317 (6.6).
+// teacher's tokens: loss and gradient of 4096 x 128256 bf16 400 us (5.2 TB/s), 4096 x 32000 fp32 170 (6.2), 4000 x 50257
+// bf16 162 (4.9), 256 x 512 with 8 tokens 7.3 us; the loss alone of 4096 x 128256 235 us (4.5), its gradient from the
+// statistics 319 (6.6). The alternatives named below were measured when the first of these took 391.
 #include <algorithm>
 #include <type_traits>
 #include "rows.cuh"
@@ -413,8 +414,8 @@ __device__ __forceinline__ void distill_auxiliary(const DistillArgs& a, DistillS
     take_entries(a, next, e);
     t = weigh<true>(a, e);
     // The first block may write sh.next[n & 1] again: a release, since nothing else orders the read before that where rows
-    // are left out. Here, while the workers have the slice; where the word is read it would hold the row up (1024 x 32000 fp32,
-    // 128 entries: 66.6 us, here 56.7).
+    // are left out. It waits for copies in flight: where the word is read, or behind the start of the next copy, 1024 x 32000
+    // fp32 with 128 entries takes 63 to 67 us, here, while the workers have the slice, 55 to 57.
     if (cluster > 1) mbar_arrive_warp_cluster(map_to_cta(&sh.taken[n & 1], 0));
     if (rank == 0 && !pass_on(n + 1)) return leave(kSiteRow);
   }

@@ -7,10 +7,10 @@
 // are off by what l and s are, relatively (2^-22 and more with V), and are held at 0, which they would pass. (maximum, l) is what
 // the backward needs. Sums are held in 32 bits, the few scalars of a row are put together in 64.
 //
-// Measured on a B200 that copies 6557 GB/s: forward 4096 x 128256 bf16 161 us (6.5 TB/s), with 20 alternatives 200, 64
-// 218, 128 243; one row 4.5 us, with 20 alternatives 7.6 (launch and the search's chain of barriers); 64 x 128256 fp32
-// 10.2 us (3.2 TB/s: a cluster's start and end are as long as its slice), with 20 alternatives 15.3. Backward 2048 x 128256
-// bf16 159 us (6.6 TB/s), 4096 rows with 64 alternatives 334.
+// Measured on a B200 that copies 6557 GB/s: forward 4096 x 128256 bf16 160 us (6.6 TB/s), with 20 alternatives 199, 64
+// 218, 128 242; one row 4.7 us, with 20 alternatives 7.9 (launch and the search's chain of barriers); 64 x 128256 fp32
+// 10.3 us (3.2 TB/s: a cluster's start and end are as long as its slice), with 20 alternatives 15.4. Backward 2048 x 128256
+// bf16 160 us (6.6 TB/s), 4096 rows with 64 alternatives 336.
 #include <algorithm>
 #include "rows.cuh"
 

@@ -95,3 +95,38 @@ def test_gradients_that_cross_the_logits_are_refused():
         distill_topk_fwd_bwd_(rows(110), values, ids, 1.0, out=rows(first))
     with pytest.raises(RuntimeError, match="overlaps"):                    # rows at another distance
         distill_topk_fwd_bwd_(rows(110), values, ids, 1.0, out=flat.as_strided((3, 100), (230, 1), 210))
+
+
+@pytest.mark.gpu
+@dtypes
+@pytest.mark.parametrize("rows", [1, 3])
+def test_the_largest_vocabulary(dtype, rows):
+    """Every form at the most columns, at an address that no vector divides: eight blocks a row with 200 KB each."""
+    import _logprobs_oracle as oracle
+    from zenyx_b200.ops import _ext
+    from zenyx_b200.ops.logprobs import MAX_TOP, MAX_VOCAB, distill_topk
+
+    V, K = MAX_VOCAB, MAX_TOP
+    flat = torch.randn(rows * (V + 1) + 1, device="cuda").mul_(3).to(dtype)
+    x = flat[1:].as_strided((rows, V), (V + 1, 1), 1)
+    y = torch.randint(0, V, (rows,), device="cuda")
+    y[-1] = V - 1
+    lp, h, top, ids, *_ = oracle.logprobs(x, y, K, 0.8)
+    a = x.detach().requires_grad_(True)
+    out = token_logprobs(a, y, top_k=K, temperature=0.8)
+    assert torch.equal(out.top_ids, ids)
+    oracle.check(out.logprobs, lp, oracle.logprob_off(lp, h, V), "logprobs")
+    oracle.check(out.entropy, h, oracle.entropy_off(h, V), "entropy")
+    g = [torch.randn(rows, device="cuda"), torch.randn(rows, device="cuda"), torch.randn(rows, K, device="cuda")]
+    (got,) = torch.autograd.grad([out.logprobs, out.entropy, out.top_logprobs], a, g)
+    oracle.check(got, *oracle.logprobs_grad(x, y, K, 0.8, *g), "gradient")
+    values = out.top_logprobs.detach() - 0.1
+    for tail in ("renormalize", "bucket"):
+        ref, grad, off, grad_off = oracle.distill(x, values, ids, 1.3, tail)
+        loss = distill_topk_fwd_bwd_(x, values, ids, 1.0, temperature=1.3, tail=tail, out=(d := torch.empty_like(got)))
+        oracle.check(loss, ref, off, "loss")
+        oracle.check(d, grad, grad_off, "gradient of the fused form")
+        loss = distill_topk(a, values, ids, temperature=1.3, tail=tail)
+        oracle.check(loss, ref, off, "loss")
+        oracle.check(torch.autograd.grad(loss.sum(), a)[0], grad, grad_off, "gradient")
+    _ext.check_status()

@@ -8,8 +8,8 @@ from zenyx_b200.ops.attention import RingContext, shard_sequence
 B, S, V, K = 2, 512, 128, 3
 
 
-def _model():
-    cfg = LlamaConfig.tiny(n_layers=2, d_model=64, n_heads=2, n_kv_heads=1, ffn_dim=96, vocab_size=V)
+def _model(n_layers=2):
+    cfg = LlamaConfig.tiny(n_layers=n_layers, d_model=64, n_heads=2, n_kv_heads=1, ffn_dim=96, vocab_size=V)
     return LlamaModel(cfg, device="cpu", dtype=torch.float32, seed=7, head_chunk_tokens=100)
 
 
@@ -64,8 +64,9 @@ def test_scores_over_a_ring_are_a_single_processs(tmp_path, world, layout):
 class _Peer:
     """A ring's buffers as the model's host code sees them (the CPU's ring does not use them)."""
 
-    def __init__(self, sequences):
+    def __init__(self, sequences, log=None):
         self.kv_shape = (sequences, S, 1, 32)
+        self.barrier = lambda: log.append("barrier")
 
 
 @pytest.mark.parametrize("sequences", [1, 2, 3])
@@ -102,3 +103,22 @@ def test_views_of_a_ring_slot_stay_inside_it():
     for bad in (lambda: ring.kv_views(0, 0, (3, 8, 1, 4)), lambda: ring.staged_kv(0, (3, 8, 1, 4)), lambda: ring.dkv_views(0, 0, (2, 9, 1, 4))):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("n_layers", [1, 2, 3])
+def test_a_slot_is_not_written_again_while_others_may_pull_from_it(monkeypatch, n_layers):
+    """Layer l uses slot l % 2 and starts with a barrier behind its write. Between a slot's use and the next write to it
+    there has to be a barrier of another layer, or one for itself."""
+    model, log = _model(n_layers), []
+    layer = model._layer_forward
+
+    def seen(l, *a, **kw):
+        log.append(l % 2)              # the write, and the barrier of ring_attn_forward behind it
+        return layer(l, *a, **kw)
+
+    monkeypatch.setattr(model, "_layer_forward", seen)
+    ring = RingContext(rank=0, degree=1, seq_len=S, peer=_Peer(1, log))
+    model.token_logprobs(torch.zeros(3, S, dtype=torch.long), ring=ring)
+    model.logits(torch.zeros(1, S, dtype=torch.long), ring)
+    assert sum(e != "barrier" for e in log) == 4 * n_layers
+    assert all(a != b for a, b in zip(log, log[1:]))

@@ -526,6 +526,10 @@ class LlamaModel(nn.Module):
             h = fused.embedding_fwd(tokens, self.w("embed.weight"))
             for l in range(self.cfg.n_layers):
                 h, _ = self._layer_forward(l, h, B, S, ring, keep=False)
+            # The last layer's K/V lie in the slot that the next pass writes first: not before every rank has pulled them.
+            # (After an even number of layers the last barrier has seen to that; a backward pass ends with one.)
+            if ring.peer is not None and self.cfg.n_layers % 2:
+                ring.peer.barrier()
             hn, _ = fused.rmsnorm_fwd(h, self.w("final_norm"), self.cfg.norm_eps)
         return hn.view(B, S, -1)
 

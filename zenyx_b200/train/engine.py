@@ -139,7 +139,8 @@ class LlamaEngine:
                      lr: Optional[float] = None, presharded: bool = False, *, temperature: float = 1.0,
                      tail: str = "renormalize", loss_scale: float = 1.0) -> torch.Tensor:
         """``train_step`` on what a teacher wrote down for the same tokens ([global_batch, seq_len, K] each, see
-        ``LlamaModel.forward_backward_distill``). Loss and gradients are ``loss_scale`` times the mean over all tokens'."""
+        ``LlamaModel.forward_backward_distill``). Loss and gradients are ``loss_scale`` times those of the
+        mean over all tokens."""
         if not presharded:
             tokens = self.shard_batch(tokens)
             teacher_logprobs, teacher_ids = self.shard_batch(teacher_logprobs), self.shard_batch(teacher_ids)
